@@ -74,12 +74,12 @@ class Target:
         return [CSRC / s for s in self.hip] + [REPO / h for h in self.headers]
 
 
-ATTENTION = Target("libfa_hip.so", ("fa_fwd.hip",), ("include/fa_hip.h",))
+ATTENTION = Target("libfa_hip.so", ("fa_fwd.hip",), ("include/fa_hip.h", "fa_amd/csrc/fa_device.h"))
 CEILING = Target("libfa_ceiling.so", ("measure/mfma_ceiling.hip",), ())
 TARGETS = (ATTENTION, CEILING)
 # Host-side sanitizers only (each -fsanitize= behind -Xarch_host): GPU code
 # is never built with them.
-HOSTSAN = Target("libfa_hip_hostsan.so", ("fa_fwd.hip",), ("include/fa_hip.h",), (
+HOSTSAN = Target("libfa_hip_hostsan.so", ATTENTION.hip, ATTENTION.headers, (
     "-g",
     "-Xarch_host", "-fsanitize=address",
     "-Xarch_host", "-fsanitize=undefined",
