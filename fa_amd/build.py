@@ -1,20 +1,24 @@
 """Build the gfx950 shared libraries with hipcc, each keyed by a content hash.
 
-Two libraries:
+Three libraries:
 
 * ``libfa_hip.so`` -- the attention forward and its C ABI
   (``fa_amd/csrc/fa_fwd.hip``, ``include/fa_hip.h``);
+* ``libfa_serve.so`` -- the serving operators and their C ABI (page plans,
+  rotary positions, paged and windowed attention:
+  ``fa_amd/csrc/serve_*.hip``, ``include/fa_serve.h``);
 * ``libfa_ceiling.so`` -- a measurement kernel that issues nothing but FP16
   MFMAs, for the board's sustained matrix rate
   (``fa_amd/csrc/measure/mfma_ceiling.hip``); never loaded by the attention
   path;
-* on request (``--sanitize``), ``libfa_hip_hostsan.so`` -- the attention
-  library with its host code (the C ABI's validation, sizing and launch
-  set-up) built with AddressSanitizer and UndefinedBehaviorSanitizer; the
-  device code is unchanged. Load it with the clang ASan runtime preloaded
+* on request (``--sanitize``), ``libfa_hip_hostsan.so`` and
+  ``libfa_serve_hostsan.so`` -- the attention and the serving library with
+  their host code (the C ABI's validation, sizing and launch set-up) built with
+  AddressSanitizer and UndefinedBehaviorSanitizer; the device code is
+  unchanged. Load it with the clang ASan runtime preloaded
   (``LD_PRELOAD=$(hipcc -print-file-name=libclang_rt.asan-x86_64.so)
   ASAN_OPTIONS=detect_leaks=0``) and point the tests at it with
-  ``FA_TEST_LIBRARY``.
+  ``FA_TEST_LIBRARY`` (``FA_TEST_SERVE_LIBRARY``).
 
 A library's build identity is the SHA-256 of every source and header it is
 compiled from and of the compiler command line (the hipcc version is recorded
@@ -75,16 +79,20 @@ class Target:
 
 
 ATTENTION = Target("libfa_hip.so", ("fa_fwd.hip",), ("include/fa_hip.h", "fa_amd/csrc/fa_device.h"))
+SERVING = Target("libfa_serve.so", ("serve_plan.hip", "serve_rotary.hip", "serve_attn.hip"),
+                 ("include/fa_serve.h", "fa_amd/csrc/fa_device.h", "fa_amd/csrc/serve_common.h"))
 CEILING = Target("libfa_ceiling.so", ("measure/mfma_ceiling.hip",), ())
-TARGETS = (ATTENTION, CEILING)
+TARGETS = (ATTENTION, SERVING, CEILING)
 # Host-side sanitizers only (each -fsanitize= behind -Xarch_host): GPU code
 # is never built with them.
-HOSTSAN = Target("libfa_hip_hostsan.so", ATTENTION.hip, ATTENTION.headers, (
+SANITIZE = (
     "-g",
     "-Xarch_host", "-fsanitize=address",
     "-Xarch_host", "-fsanitize=undefined",
     "-Xarch_host", "-fno-omit-frame-pointer",
-))
+)
+HOSTSAN = Target("libfa_hip_hostsan.so", ATTENTION.hip, ATTENTION.headers, SANITIZE)
+SERVING_HOSTSAN = Target("libfa_serve_hostsan.so", SERVING.hip, SERVING.headers, SANITIZE)
 
 # The attention library (what the product path loads).
 LIBRARY = ATTENTION.library
@@ -177,11 +185,12 @@ def main(argv=None):
     ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     ap.add_argument("--force", action="store_true", help="rebuild even when up to date")
     ap.add_argument("--sanitize", action="store_true",
-                    help="also build libfa_hip_hostsan.so (host code under ASan and UBSan)")
+                    help="also build the *_hostsan.so libraries (host code under ASan and UBSan)")
     args = ap.parse_args(argv)
     build_all(force=args.force, verbose=True)
     if args.sanitize:
-        build(force=args.force, verbose=True, target=HOSTSAN)
+        for target in (HOSTSAN, SERVING_HOSTSAN):
+            build(force=args.force, verbose=True, target=target)
 
 
 if __name__ == "__main__":

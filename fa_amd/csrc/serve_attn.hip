@@ -1,0 +1,1637 @@
+// Attention of new tokens over a paged cache, and with a causal sliding window
+// and sinks, paged or contiguous: GQA, 128 dims, FP16 or BF16, FP32 softmax
+// statistics and O.
+//
+// A request has n new rows per head behind its earlier keys; row i stands at
+// position p and sees key j iff j <= p and (j > p - W or j < S). One pass over
+// the keys per row, with the running maximum m and sum l of the softmax (base
+// 2, scale folded in, c = scale log2 e):
+//   m' = max(m, max_j s_j), a = 2^((m - m') c), P_j = 2^(s_j c - m' c),
+//   l' = a l + sum_j P_j, O' = a O + sum_j P_j v_j,
+// at the end o = O / l, lse = ln l + scale m.
+//
+// Rows are packed: the n * group rows of the query heads that share a KV head
+// form one sequence, position by position, of which a tile is a run of
+// consecutive rows. A tile needs keys [0, min(S, hi)) and [lo, hi), lo the first key
+// its first row's window holds and hi one past its last row's position: a list
+// of 128-key blocks, the blocks that all its rows see whole and those that take
+// the mask. A block's keys may lie in any pages: the loads from a 16-key
+// group, which no page end cuts, go through a buffer descriptor of its own,
+// with the page's address as a 64-bit base and its range ending behind the
+// request's last key. So caches may be of any size, and what lies behind the
+// last key is never read: it arrives in LDS as zeros.
+//
+// Matrix products run transposed, S^T = K Q^T and O^T += V^T P^T, so that a lane
+// holds one row's scores and sums; the P^T operand is the S^T registers,
+// converted, and V^T comes from V in its natural layout through transposing LDS
+// reads (v_mfma 32x32x16, ds_read_b64_tr_b16; operand layouts at `Fragments`).
+//
+// A key that the mask hides has its score replaced by -inf, so NaN in its K has
+// no effect; NaN or an infinity in its V would get into O through the product
+// 0 * NaN in the blocks that take the mask. That is found at the end (l is a
+// number and O is not) and the row computed again key by key (repair_row).
+
+#include <math.h>
+
+#include <algorithm>
+#include <atomic>
+#include <initializer_list>
+
+#include "fa_device.h"
+#include "serve_common.h"
+
+namespace {
+
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int HD = 128;
+constexpr int ROW_BYTES = HD * 2;
+constexpr int BLOCK = 128;                  // keys of a block of the lists below
+constexpr double LOG2E = 1.4426950408889634;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr int NO_WINDOW = 1 << 30;
+// The maximum is raised when a score exceeds it by more than this (in powers of
+// two), so P <= 2^8 and O is rescaled rarely.
+constexpr float TAU = 8.f;
+
+struct AttnArgs {
+  const char *q, *k, *v;
+  char* o;
+  float* lse;
+  const int *table, *starts, *lengths;      // paged; null: contiguous
+  int64_t table_stride;
+  int64_t qs_b, qs_n, qs_h, os_b, os_n, os_h;             // byte strides of q and o
+  int64_t ks_b, vs_b, ks_h, vs_h;                         // of a page (or batch entry), a head
+  int ks_n, vs_n;                                         // of a key
+  int64_t ls_b, ls_n, ls_h;                               // strides of lse
+  int batch, heads_kv, group, tokens, pages, shift, max_pages;
+  int seq_q, seq_k, off;                    // contiguous: lengths, position of row 0
+  int window, sinks;
+  float c;
+  int rows_max;                             // packed rows of a request that the row kernel takes
+  int split;                                // tile kernel: there is room for parts
+  float *opart, *lpart;                     // row kernel's parts
+  int* desc;
+  float *topart, *tlpart;                   // tile kernel's parts
+  int* tdesc;
+  int groups;                               // workgroups of the row kernel
+};
+
+// A value every lane of the wave has, in a scalar register (integer divisions, for
+// one, are made in vector registers).
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ uint64_t uniform(uint64_t x) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) |
+         (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
+}
+
+// A batch entry: the first of its rows in q, their number, the position of
+// row 0, its keys, and whether its table row is too short for them.
+struct Request {
+  int row0, n, pos, keys;
+  bool bad;
+};
+template <bool PAGED>
+__device__ __forceinline__ Request request(const AttnArgs& a, int b) {
+  Request r;
+  if constexpr (PAGED) {
+    const int s0 = min(max(a.starts[b], 0), a.tokens), s1 = min(max(a.starts[b + 1], s0), a.tokens);
+    const int len = max(a.lengths[b], 0);
+    const int64_t cap = (int64_t)a.max_pages << a.shift;
+    r.row0 = s0;
+    r.n = s1 - s0;
+    r.pos = len - r.n;
+    r.bad = len > cap;
+    r.keys = r.bad ? (int)cap : len;
+  } else {
+    r.row0 = 0;
+    r.n = a.seq_q;
+    r.pos = a.off;
+    r.keys = a.seq_k;
+    r.bad = false;
+  }
+  return r;
+}
+
+// The request of a whole workgroup, in scalar registers: descriptors and loop
+// bounds are made from it.
+template <bool PAGED>
+__device__ __forceinline__ Request uniform_request(const AttnArgs& a, int b) {
+  Request r = request<PAGED>(a, b);
+  if constexpr (PAGED) {
+    r.row0 = __builtin_amdgcn_readfirstlane(r.row0);
+    r.n = __builtin_amdgcn_readfirstlane(r.n);
+    r.pos = __builtin_amdgcn_readfirstlane(r.pos);
+    r.keys = __builtin_amdgcn_readfirstlane(r.keys);
+    r.bad = __builtin_amdgcn_readfirstlane((int)r.bad);
+  }
+  return r;
+}
+
+// The key blocks that rows at positions first .. last see: blocks [0, ns) and
+// [w0, w1), of which [f0, f1) (within [w0, w1)) are seen whole by every row.
+struct Blocks {
+  int ns, w0, w1, f0, f1;
+  __device__ __forceinline__ int total() const { return ns + w1 - w0; }
+};
+__device__ __forceinline__ Blocks blocks(const AttnArgs& a, const Request& r, int first, int last) {
+  Blocks k;
+  const int hi = min(last + 1, r.keys);
+  if (hi <= 0) return Blocks{0, 0, 0, 0, 0};
+  const int lo = min(max(first - a.window + 1, 0), hi);
+  k.w0 = lo / BLOCK;
+  k.w1 = (hi + BLOCK - 1) / BLOCK;
+  if (lo == hi) k.w0 = k.w1;
+  k.ns = min((min(a.sinks, hi) + BLOCK - 1) / BLOCK, k.w0);
+  // Whole for all: from the last row's window start to the first row's position.
+  const int full_hi = min(first + 1, r.keys), full_lo = max(last - a.window + 1, 0);
+  k.f0 = min(max((full_lo + BLOCK - 1) / BLOCK, k.w0), k.w1);
+  k.f1 = max(min(full_hi > 0 ? full_hi / BLOCK : 0, k.w1), k.f0);
+  return k;
+}
+
+// ---------------------------------------------------------------------------
+// Fragments. The 32x32 output layout gives lane l column l % 32 and rows
+// 8g + 4(l / 32) + e (register 4g + e): of S^T, query row l % 32 and those keys.
+// The PV step over keys 16s .. 16s + 15 takes P^T from registers 8s .. 8s + 7
+// converted, so its k slots 8h .. 8h + 7 (h = l / 32) hold keys 16s + 4h + {0..3}
+// and 16s + 8 + 4h + {0..3}; the V^T operand follows that order with two
+// transposing reads of 4 keys each.
+template <bool BF>
+__device__ __forceinline__ f32x16 mma(h8 x, h8 y, f32x16 acc) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, x), __builtin_bit_cast(b8, y), acc,
+                                                   0, 0, 0);
+  else
+    return mfma32(x, y, acc);
+}
+// Two probabilities rounded to the element type (the matrix operand), as one word.
+// l sums them unrounded: it becomes the FP32 log-sum-exp, and rounding P to 8 or
+// 11 bits leaves O = sum P16 v / l off by at most half a step of the type times
+// sum P |v| / l, the size of its own rounding at the end.
+template <bool BF>
+__device__ __forceinline__ uint32_t pack_p(float p0, float p1) {
+  if constexpr (BF)
+    return __builtin_bit_cast(uint32_t, b2{(__bf16)p0, (__bf16)p1});
+  else
+    return __builtin_bit_cast(uint32_t, h2{(_Float16)p0, (_Float16)p1});
+}
+template <bool BF>
+__device__ __forceinline__ float widen(uint16_t x) {
+  if constexpr (BF)
+    return __uint_as_float((uint32_t)x << 16);
+  else
+    return (float)__builtin_bit_cast(_Float16, x);
+}
+template <bool BF>
+__device__ __forceinline__ uint16_t narrow(float x) {
+  if constexpr (BF)
+    return __builtin_bit_cast(uint16_t, (__bf16)x);
+  else
+    return __builtin_bit_cast(uint16_t, (_Float16)x);
+}
+
+// A score, or -inf for a key outside [.., hi] or outside both [lo, ..] and
+// [.., sink) (all relative to the same key). Sign arithmetic and a bit select:
+// compares and selects would keep a scalar register pair per score alive.
+__device__ __forceinline__ float masked(float s, int key, int hi, int lo, int sink) {
+  const int hidden = min(hi - key, max(key - lo, sink - 1 - key)) >> 31;
+  const uint32_t bits = __float_as_uint(s);
+  return __uint_as_float((bits & ~(uint32_t)hidden) | (0xff800000u & (uint32_t)hidden));
+}
+
+// One step of the online softmax over N scores of the lane's row (the other
+// half of the keys is with lane + 32): raises m, rescales l and O if some row of
+// the wave needs it, and turns the scores into P fragments. at(i) runs before
+// the exponentials of pair i.
+template <bool BF, int T, typename At>
+__device__ __forceinline__ void softmax_step(f32x16 (&s)[T], h8 (&p)[2 * T], float& m, float& l,
+                                             f32x16 (&acc)[4], float c, At&& at) {
+  float mv[16 * T];
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mv[16 * t + r] = s[t][r];
+#pragma unroll
+  for (int n = 16 * T; n > 1; n = (n + 2) / 3) {
+#pragma unroll
+    for (int i = 0; 3 * i < n; ++i) {
+      float x = mv[3 * i];
+      if (3 * i + 1 < n) x = smax(x, mv[3 * i + 1]);
+      if (3 * i + 2 < n) x = smax(x, mv[3 * i + 2]);
+      mv[i] = x;
+    }
+  }
+  const float mx = half_max(mv[0]);
+  // False where both are -inf (no key seen yet) and for NaN, which then shows in P.
+  const bool need = (mx - m) * c > TAU;
+  if (__builtin_amdgcn_ballot_w64(need)) {
+    const float alpha = need ? __builtin_amdgcn_exp2f((m - mx) * c) : 1.f;
+    m = need ? mx : m;
+    l *= alpha;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) acc[dt] *= alpha;
+  }
+  const float mc = m == -INFINITY ? 0.f : m * c;
+  float ls[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      u32x4 frag;
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        at((2 * t + g) * 4 + e / 2);
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][8 * g + e], c, -mc));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][8 * g + e + 1], c, -mc));
+        frag[e / 2] = pack_p<BF>(p0, p1);
+        ls[e & 2] += p0;
+        ls[(e & 2) + 1] += p1;
+      }
+      p[2 * t + g] = __builtin_bit_cast(h8, frag);
+    }
+  l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+}
+
+// Keys of one KV head of a request: descriptors for the loads of a 16-key group.
+template <bool PAGED>
+struct Stream {
+  const char *k, *v;                        // of the head
+  const int __attribute__((address_space(4)))* table;     // the request's row
+  uint32_t ks_b, vs_b;
+  int ks_n, vs_n, keys, pages, shift;
+  __device__ __forceinline__ Stream(const AttnArgs& a, const Request& r, int b, int hk) {
+    k = a.k + hk * a.ks_h;
+    v = a.v + hk * a.vs_h;
+    if constexpr (PAGED) {
+      table = (const int __attribute__((address_space(4)))*)(uintptr_t)(a.table + b * a.table_stride);
+      ks_b = (uint32_t)a.ks_b;
+      vs_b = (uint32_t)a.vs_b;
+    } else {
+      k += b * a.ks_b;
+      v += b * a.vs_b;
+    }
+    ks_n = a.ks_n;
+    vs_n = a.vs_n;
+    keys = r.keys;
+    pages = a.pages;
+    shift = a.shift;
+  }
+  // The page of the group at `key` (for a group past the last key, of that key).
+  __device__ __forceinline__ int page(int key) const {
+    if constexpr (PAGED)
+      return __builtin_amdgcn_readfirstlane(table[max(min(key, keys - 1), 0) >> shift]);
+    else
+      return 0;
+  }
+  // Keys of the group at `key` that may be read: none if the page does not exist.
+  __device__ __forceinline__ int valid(int key, int id) const {
+    int n = min(max(keys - key, 0), 16);
+    if constexpr (PAGED) n = (uint32_t)id < (uint32_t)pages ? n : 0;
+    return n;
+  }
+  __device__ __forceinline__ bool missing(int key, int id) const {
+    return PAGED && key < keys && (uint32_t)id >= (uint32_t)pages;
+  }
+  __device__ __forceinline__ i32x4 rsrc(const char* base, uint32_t page_bytes, int pitch, int key, int id) const {
+    const int n = valid(key, id);
+    if constexpr (PAGED)
+      base += (uint64_t)(uint32_t)id * page_bytes + (uint64_t)(uint32_t)(key & ((1 << shift) - 1)) * (uint32_t)pitch;
+    else
+      base += (int64_t)key * pitch;
+    return buffer_rsrc(n ? base : nullptr, n ? (n - 1) * pitch + ROW_BYTES : 0);
+  }
+  __device__ __forceinline__ i32x4 k_rsrc(int key, int id) const { return rsrc(k, ks_b, ks_n, key, id); }
+  __device__ __forceinline__ i32x4 v_rsrc(int key, int id) const { return rsrc(v, vs_b, vs_n, key, id); }
+  // A key's row (a key the request has, in a page that exists).
+  __device__ __forceinline__ int64_t at(int key, int64_t page_bytes, int pitch) const {
+    if constexpr (PAGED)
+      return table[key >> shift] * page_bytes + (int64_t)(key & ((1 << shift) - 1)) * pitch;
+    else
+      return (int64_t)key * pitch;
+  }
+};
+
+// A row again, one key at a time, over the blocks [s0, s1) of a list: o (dims
+// 2 lane, 2 lane + 1) and lse of the keys it sees, which alone are read. The
+// whole wave works on one row; for the rare rows that NaN in a hidden key's V
+// has reached.
+template <bool BF, bool PAGED, typename BlockAt>
+__device__ __forceinline__ void repair_row(const AttnArgs& a, const Stream<PAGED>& st, const char* qrow, int pos,
+                                           int s0, int s1, BlockAt&& block_at, float (&o)[2], float& lse) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t qw = *reinterpret_cast<const uint32_t*>(qrow + 4 * lane);
+  const float q0 = widen<BF>((uint16_t)qw), q1 = widen<BF>((uint16_t)(qw >> 16));
+  float m = -INFINITY, l = 0.f;
+  o[0] = o[1] = 0.f;
+  const int hi = min(pos, st.keys - 1);
+  for (int s = s0; s < s1; ++s) {
+    const int key0 = block_at(s) * BLOCK;
+    for (int key = key0; key < key0 + BLOCK && key <= hi; ++key) {
+      if (key <= pos - a.window && key >= a.sinks) continue;
+      const uint32_t kw = *reinterpret_cast<const uint32_t*>(st.k + st.at(key, a.ks_b, a.ks_n) + 4 * lane);
+      const uint32_t vw = *reinterpret_cast<const uint32_t*>(st.v + st.at(key, a.vs_b, a.vs_n) + 4 * lane);
+      float x = __builtin_fmaf(q0, widen<BF>((uint16_t)kw), q1 * widen<BF>((uint16_t)(kw >> 16)));
+#pragma unroll
+      for (int d = 32; d >= 1; d >>= 1) x += __shfl_xor(x, d);
+      if ((x - m) * a.c > TAU) {
+        const float alpha = __builtin_amdgcn_exp2f((m - x) * a.c);
+        m = x;
+        l *= alpha;
+        o[0] *= alpha;
+        o[1] *= alpha;
+      }
+      const float p = __builtin_amdgcn_exp2f(m == -INFINITY ? x * a.c : (x - m) * a.c);
+      l += p;
+      o[0] = __builtin_fmaf(p, widen<BF>((uint16_t)vw), o[0]);
+      o[1] = __builtin_fmaf(p, widen<BF>((uint16_t)(vw >> 16)), o[1]);
+    }
+  }
+  const float inv = l > 0.f ? 1.f / l : l;  // NaN stays
+  o[0] *= inv;
+  o[1] *= inv;
+  lse = (__builtin_amdgcn_logf(l) + m * a.c) * LN2;
+}
+
+__device__ __forceinline__ bool is_nan(float x) { return !(x == x); }
+
+// ---------------------------------------------------------------------------
+// The row kernel: requests of few rows (decode, a few tokens behind a cache).
+// Every key is read once and that read is the bound, so the kernel is laid out
+// for bytes in flight and even shares. A workgroup is 4 waves, two of them to a CU
+// (64 KiB of LDS each); a wave takes 32 of a block's 128 keys for itself, its own
+// LDS slots (8 KiB of K, 8 KiB of V), statistics and O, so the key loop has no
+// barrier: K(j + 1) is loaded once K(j) is in registers, V(j + 1) after the
+// products of block j. The four results are joined in LDS at an item's end.
+//
+// An item is a 32-row tile of one KV head of a request. The blocks of all items,
+// in order, are one long axis of which each workgroup takes an equal share,
+// whatever the requests' lengths; a share starts and ends anywhere in an item. A
+// piece of an item leaves its normalised O and lse in the workspace (a
+// workgroup has at most two, its first and its last), and the merge kernel joins
+// an item's pieces.
+constexpr int RT = 32;
+constexpr int RW = 4;                       // waves
+constexpr int RTHREADS = RW * 64;
+constexpr int RSLOT = 32 * ROW_BYTES;       // 32 keys of K or V
+constexpr int kRowsLds = RW * 2 * RSLOT;
+constexpr int kRowsGroups = 512;            // two a CU
+constexpr int kMinShare = 2;                // blocks a share holds at least
+constexpr int DESC_INTS = 8;                // ints of a descriptor
+
+struct Piece {
+  int b, hk, tile, first, last;             // item, and the workgroups that share it
+};
+
+template <bool PAGED>
+__device__ __forceinline__ int row_tiles(const AttnArgs& a, const Request& r) {
+  const int64_t rows = (int64_t)r.n * a.group;
+  return rows <= a.rows_max ? (int)((rows + RT - 1) / RT) : 0;
+}
+// Blocks of every item of a request: those any of its rows sees, at least one (an
+// item whose rows see nothing still writes zeros).
+__device__ __forceinline__ int row_blocks(const AttnArgs& a, const Request& r) {
+  return max(blocks(a, r, r.pos, r.pos + r.n - 1).total(), 1);
+}
+
+__device__ __forceinline__ Blocks uniform(const Blocks& k) {
+  return Blocks{uniform(k.ns), uniform(k.w0), uniform(k.w1), uniform(k.f0), uniform(k.f1)};
+}
+
+template <bool BF, bool PAGED>
+__device__ __forceinline__ void row_item(const AttnArgs& a, const Request& r, int b, int hk, int tile, int s0, int s1,
+                                         int nblk, int slot, char* lds, float* st_m, float* st_l) {
+  // Opaque, so that nothing derived from it is kept across the items.
+  int tid;
+  asm volatile("v_mov_b32 %0, %1" : "=v"(tid) : "v"((int)threadIdx.x));
+  const int lane = tid & 63, l32 = lane & 31, hf = lane >> 5, lr = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rows = r.n * a.group;
+  const int row = min(tile * RT + l32, rows - 1);
+  const int i = row / a.group, head = hk * a.group + row % a.group;
+  const int pos = r.pos + i;
+  const Blocks bl = uniform(blocks(a, r, r.pos, r.pos + r.n - 1));
+  auto block_at = [&](int s) { return s < bl.ns ? s : bl.w0 + s - bl.ns; };
+  // Whether the keys [key, key + 32) are seen whole by every row of the tile.
+  const int first = uniform(r.pos + tile * RT / a.group);
+  const int last = uniform(r.pos + min(tile * RT + RT - 1, rows - 1) / a.group);
+  auto whole = [&](int key) {
+    return key + 31 <= min(first, r.keys - 1) && (key > last - a.window || key + 32 <= a.sinks);
+  };
+  const Stream<PAGED> st(a, r, b, hk);
+
+  // A load instruction fills 4 rows of 256 bytes: lane l brings row l / 16, the
+  // chunk its place holds. K keeps chunk c of row n at c ^ n % 16 (the 32 rows
+  // an operand read takes one chunk column from then lie in different banks), V
+  // at c ^ 4 (n % 4) (a transposing read's 4 rows in the 4 quarters of the banks).
+  int koff[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) koff[x] = lr * st.ks_n + ((lane & 15) ^ (4 * x + lr)) * 16;
+  const int voff = lr * st.vs_n + ((lane & 15) ^ (4 * lr)) * 16;
+  char* kslot = lds + wave * 2 * RSLOT;
+  char* vslot = kslot + RSLOT;
+  const uint32_t kdst = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)kslot;
+  const uint32_t vdst = kdst + RSLOT;
+  bool bad = r.bad;
+  // Keys of this wave in block s of the list (past the piece: no keys).
+  auto key_of = [&](int s) { return s < s1 ? block_at(s) * BLOCK + wave * 32 : 1 << 30; };
+  auto load_k = [&](int key, const int (&id)[2]) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      bad |= st.missing(key + 16 * g, id[g]);
+      const i32x4 rs = st.k_rsrc(key + 16 * g, id[g]);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) dma_to_lds(rs, kdst + (4 * g + x) * 1024, koff[x], 4 * x * st.ks_n);
+    }
+  };
+  auto load_v = [&](int key, const int (&id)[2]) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const i32x4 rs = st.v_rsrc(key + 16 * g, id[g]);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) dma_to_lds(rs, vdst + (4 * g + x) * 1024, voff, 4 * x * st.vs_n);
+    }
+  };
+  auto pages_of = [&](int key, int (&id)[2]) {
+    id[0] = st.page(key);
+    id[1] = st.page(key + 16);
+  };
+
+  const char* qrow = a.q + b * a.qs_b + (int64_t)(r.row0 + i) * a.qs_n + head * a.qs_h;
+  int id[2], next[2];
+  int key = key_of(s0);
+  pages_of(key, id);
+  h8 qf[8];
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) qf[kk] = *reinterpret_cast<const h8*>(qrow + (kk * 2 + hf) * 16);
+  load_k(key, id);
+  load_v(key, id);
+  int key_next = key_of(s0 + 1);
+  pages_of(key_next, next);
+  // The compiler waits for its own loads here, before the key loop.
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) asm volatile("" ::"v"(qf[kk]));
+
+  const int k_lane = l32 * ROW_BYTES + ((hf ^ (l32 & 15)) << 4);
+  int v_lane[4];
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt) {
+    const int e = (lane & 15) >> 2;
+    v_lane[dt] = (4 * hf + e) * ROW_BYTES + (4 * (dt ^ e) + 2 * (lr & 1) + ((lane & 3) >> 1)) * 16 + (lane & 1) * 8;
+  }
+  f32x16 acc[4];
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt) acc[dt] = f32x16{};
+  float m = -INFINITY, l = 0.f;
+  for (int s = s0; s < s1; ++s) {
+    wait_loads<8>();                        // K has landed; V may be in flight
+    f32x16 sc[1];
+    sc[0] = f32x16{};
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk)
+      sc[0] = mma<BF>(*reinterpret_cast<const h8*>(kslot + (k_lane ^ (kk << 5))), qf[kk], sc[0]);
+    wait_lds();
+    load_k(key_next, next);
+    if (!whole(key)) {
+      const int base = key + 4 * hf;
+      const int hi = min(pos, r.keys - 1) - base, lo = pos - a.window + 1 - base, sink = a.sinks - base;
+#pragma unroll
+      for (int x = 0; x < 16; ++x) sc[0][x] = masked(sc[0][x], 8 * (x >> 2) + (x & 3), hi, lo, sink);
+    }
+    h8 p[2];
+    softmax_step<BF, 1>(sc, p, m, l, acc, a.c, [](int) {});
+    wait_loads<8>();                        // V has landed; the next K may be in flight
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) {
+        const char* at = vslot + v_lane[dt] + ks * 16 * ROW_BYTES;
+        const h8 x = __builtin_shufflevector(lds_read_tr(at), lds_read_tr(at + 8 * ROW_BYTES), 0, 1, 2, 3, 4, 5, 6, 7);
+        acc[dt] = mma<BF>(x, p[ks], acc[dt]);
+      }
+    wait_lds();
+    load_v(key_next, next);
+    key = key_next;
+    key_next = key_of(s + 2);
+    pages_of(key_next, next);
+  }
+
+  // Join the waves: O goes to the wave's own 16 KiB of slots once its loads have
+  // landed, 512-byte rows with chunk c of row n at c ^ n, m and l beside them.
+  wait_loads<0>();
+  const float lw = bad ? NAN : half_sum(l);
+  if (hf == 0) {
+    st_m[wave * RT + l32] = m;
+    st_l[wave * RT + l32] = lw;
+  }
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float4 val = {acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
+      *reinterpret_cast<float4*>(kslot + l32 * 512 + (((dt * 8 + 2 * g + hf) ^ l32) << 4)) = val;
+    }
+  __syncthreads();
+  // 8 threads a row, 16 dims each: 8 at 8t and 8 at 64 + 8t.
+  const int n = tid >> 3, t = tid & 7;
+  const int orow = tile * RT + n;
+  float M = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < RW; ++w) M = smax(M, st_m[w * RT + n]);
+  float L = 0.f, o[16];
+#pragma unroll
+  for (int x = 0; x < 16; ++x) o[x] = 0.f;
+#pragma unroll
+  for (int w = 0; w < RW; ++w) {
+    const float mw = st_m[w * RT + n];
+    const float f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw - M) * a.c);
+    L = __builtin_fmaf(f, st_l[w * RT + n], L);
+    const char* base = lds + w * 2 * RSLOT + n * 512;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int chunk = (x >> 1) * 16 + 2 * t + (x & 1);
+      const float4 val = *reinterpret_cast<const float4*>(base + ((chunk ^ n) << 4));
+      o[4 * x] = __builtin_fmaf(f, val.x, o[4 * x]);
+      o[4 * x + 1] = __builtin_fmaf(f, val.y, o[4 * x + 1]);
+      o[4 * x + 2] = __builtin_fmaf(f, val.z, o[4 * x + 2]);
+      o[4 * x + 3] = __builtin_fmaf(f, val.w, o[4 * x + 3]);
+    }
+  }
+  __syncthreads();                          // the slots may be filled again
+  const bool inside = orow < rows;
+  const int orc = inside ? orow : rows - 1;
+  const int oi = orc / a.group, ohead = hk * a.group + orc % a.group;
+  const bool part = s0 > 0 || s1 < nblk;
+  float* prow = a.opart + ((int64_t)slot * RT + n) * HD;
+  char* out = a.o + b * a.os_b + (int64_t)(r.row0 + oi) * a.os_n + ohead * a.os_h;
+  float* out_lse = a.lse + b * a.ls_b + (int64_t)(r.row0 + oi) * a.ls_n + ohead * a.ls_h;
+  // O is not a number though every weight is: a hidden key's V (see above).
+  float sum = 0.f;
+#pragma unroll
+  for (int x = 0; x < 16; ++x) sum += o[x] * 0.f;
+  uint64_t sick = __builtin_amdgcn_ballot_w64(inside && is_nan(sum) && !is_nan(L));
+  bool again = false;
+  while (sick) {
+    const int at = __ffsll((unsigned long long)sick) - 1;
+    sick &= ~(0xffull << (at & ~7));
+    again |= (lane >> 3) == (at >> 3);
+    const int row = tile * RT + __builtin_amdgcn_readfirstlane(__shfl(n, at));
+    const int ri = row / a.group, rh = hk * a.group + row % a.group;
+    float x[2], rl;
+    repair_row<BF, PAGED>(a, st, a.q + b * a.qs_b + (int64_t)(r.row0 + ri) * a.qs_n + rh * a.qs_h, r.pos + ri, s0, s1,
+                          block_at, x, rl);
+    if (part) {
+      float* dst = a.opart + ((int64_t)slot * RT + row - tile * RT) * HD;
+      dst[2 * lane] = x[0];
+      dst[2 * lane + 1] = x[1];
+      if (lane == 0) a.lpart[(int64_t)slot * RT + row - tile * RT] = rl;
+    } else {
+      char* dst = a.o + b * a.os_b + (int64_t)(r.row0 + ri) * a.os_n + rh * a.os_h;
+      *reinterpret_cast<uint32_t*>(dst + 4 * lane) = narrow<BF>(x[0]) | (uint32_t)narrow<BF>(x[1]) << 16;
+      if (a.lse && lane == 0) a.lse[b * a.ls_b + (int64_t)(r.row0 + ri) * a.ls_n + rh * a.ls_h] = rl;
+    }
+  }
+  if (!inside || again) return;
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const float lse = (__builtin_amdgcn_logf(L) + M * a.c) * LN2;
+  if (part) {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int chunk = (x >> 1) * 16 + 2 * t + (x & 1);
+      *reinterpret_cast<float4*>(prow + 4 * chunk) =
+          float4{o[4 * x] * inv, o[4 * x + 1] * inv, o[4 * x + 2] * inv, o[4 * x + 3] * inv};
+    }
+    if (t == 0) a.lpart[(int64_t)slot * RT + n] = lse;
+  } else {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      u16x8 val;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) val[e] = narrow<BF>(o[8 * x + e] * inv);
+      *reinterpret_cast<u16x8*>(out + (64 * x + 8 * t) * 2) = val;
+    }
+    if (a.lse && t == 0) *out_lse = lse;
+  }
+}
+
+template <bool BF, bool PAGED>
+__global__ void __launch_bounds__(RTHREADS) __attribute__((amdgpu_waves_per_eu(2, 2)))
+fa_serve_rows_kernel(AttnArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ float st_m[RW * RT], st_l[RW * RT];
+  __shared__ uint32_t wave_sum[RW];
+  __shared__ int found[2];
+  __shared__ uint32_t found_at;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // Blocks of all items before this thread's run of requests, and of all.
+  const int per = (a.batch + RTHREADS - 1) / RTHREADS;
+  const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
+  auto cost = [&](const Request& r) {
+    const int tiles = row_tiles<PAGED>(a, r);
+    return tiles ? (uint32_t)(a.heads_kv * tiles * row_blocks(a, r)) : 0u;
+  };
+  uint32_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += cost(request<PAGED>(a, b));
+  uint32_t sum = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t other = __shfl_up(sum, d);
+    if (lane >= d) sum += other;
+  }
+  if (lane == 63) wave_sum[wave] = sum;
+  __syncthreads();
+  uint32_t before = sum - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < RW; ++w) {
+    if (w < wave) before += wave_sum[w];
+    total += wave_sum[w];
+  }
+  const int g = blockIdx.x;
+  total = uniform(total);
+  const uint32_t share = max(uniform((total + a.groups - 1) / a.groups), (uint32_t)kMinShare);
+  uint32_t x = share * g;
+  const uint32_t end = min(x + share, total);
+  int* desc = a.desc + g * DESC_INTS;
+  if (tid == 0) desc[3] = -1;               // no item that began earlier, so far
+  if (x >= total) return;                   // uniform
+  if (tid == 0) found[0] = a.batch;
+  __syncthreads();
+  if (before <= x && x < before + mine) {
+    int b = b0;
+    uint32_t at = before;
+    for (;; ++b) {
+      const uint32_t n = cost(request<PAGED>(a, b));
+      if (x < at + n) break;
+      at += n;
+    }
+    found[0] = b;
+    found_at = at;
+  }
+  __syncthreads();
+  int b = __builtin_amdgcn_readfirstlane(found[0]);
+  uint32_t at = uniform(found_at);          // where request b's blocks start
+  bool head = true;
+  for (; b < a.batch; ++b) {
+    const Request r = uniform_request<PAGED>(a, b);
+    const int tiles = row_tiles<PAGED>(a, r);
+    if (tiles) {
+      const int nblk = uniform(row_blocks(a, r));
+      const uint32_t stop = at + (uint32_t)a.heads_kv * tiles * nblk;
+      while (x < end && x < stop) {
+        const uint32_t rel = x - at, item = uniform(rel / (uint32_t)nblk);
+        const int s0 = uniform((int)(rel - item * (uint32_t)nblk));
+        const int s1 = uniform((int)min((uint32_t)nblk, s0 + (end - x)));
+        const int hk = uniform((int)(item / (uint32_t)tiles)), tile = uniform((int)(item - (uint32_t)hk * tiles));
+        if (head && s0 > 0 && tid == 0) {
+          // The workgroups that share an item that began before this one's share.
+          const uint32_t start = x - s0;
+          desc[0] = b;
+          desc[1] = hk;
+          desc[2] = tile;
+          desc[3] = (int)(start / share);
+          desc[4] = (int)((start + nblk - 1) / share);
+        }
+        head = false;
+        row_item<BF, PAGED>(a, r, b, hk, tile, s0, s1, nblk, 2 * g + (s0 == 0), lds, st_m, st_l);
+        x += s1 - s0;
+      }
+      at = stop;
+    }
+    if (x >= end) break;
+  }
+}
+
+// Joins the pieces of the items that several workgroups share:
+//   O = sum w_s O_s / sum w_s, w_s = exp(lse_s - M), M = max lse_s, lse = M + ln sum w_s.
+// Workgroup g > 0 whose share starts inside an item is one of the K that do; the
+// j-th of them takes rows j, j + K, .. of the item's 32, so a launch's joins are
+// spread evenly however many pieces an item has. A row's pieces are read by 8
+// groups of 32 lanes, 4 dims a lane, and joined in LDS.
+template <bool BF, bool PAGED>
+__global__ void __launch_bounds__(256) fa_serve_rows_merge_kernel(AttnArgs a) {
+  __shared__ float weight[kRowsGroups];
+  __shared__ float red[8][HD];
+  __shared__ float wave_red[4];
+  const int* desc = a.desc + (blockIdx.x + 1) * DESC_INTS;
+  const int first = desc[3];
+  if (first < 0) return;
+  const int b = desc[0], hk = desc[1], tile = desc[2], last = desc[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int boundaries = last - first, pieces = boundaries + 1;
+  const Request r = request<PAGED>(a, b);
+  const int rows = min(r.n * a.group - tile * RT, RT);
+  auto piece = [&](int s) { return (int64_t)(2 * (first + s) + (s == 0)); };
+  for (int n = (int)blockIdx.x - first; n < rows; n += boundaries) {
+    float mine = -INFINITY;
+    for (int s = tid; s < pieces; s += 256) mine = smax(mine, a.lpart[piece(s) * RT + n]);
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) mine = smax(mine, __shfl_xor(mine, d));
+    __syncthreads();                        // the last row's LDS has been read
+    if (lane == 0) wave_red[wave] = mine;
+    __syncthreads();
+    const float M = smax(smax(wave_red[0], wave_red[1]), smax(wave_red[2], wave_red[3]));
+    __syncthreads();
+    float total = 0.f;
+    for (int s = tid; s < pieces; s += 256) {
+      const float x = a.lpart[piece(s) * RT + n];
+      const float w = x == -INFINITY ? 0.f : expf(x - M);
+      weight[s] = w;
+      total += w;
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) total += __shfl_xor(total, d);
+    if (lane == 0) wave_red[wave] = total;
+    __syncthreads();
+    total = (wave_red[0] + wave_red[1]) + (wave_red[2] + wave_red[3]);
+    const int grp = tid >> 5, dim = (tid & 31) * 4;
+    float4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = grp; s < pieces; s += 8) {
+      const float w = weight[s];
+      const float4 v = *reinterpret_cast<const float4*>(a.opart + (piece(s) * RT + n) * HD + dim);
+      if (w != 0.f) {                       // a piece without keys may hold NaN
+        o.x = __builtin_fmaf(w, v.x, o.x);
+        o.y = __builtin_fmaf(w, v.y, o.y);
+        o.z = __builtin_fmaf(w, v.z, o.z);
+        o.w = __builtin_fmaf(w, v.w, o.w);
+      }
+    }
+    *reinterpret_cast<float4*>(&red[grp][dim]) = o;
+    __syncthreads();
+    if (tid < 64) {
+      float x[2] = {0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        x[0] += red[s][2 * tid];
+        x[1] += red[s][2 * tid + 1];
+      }
+      const float inv = total == 0.f ? 0.f : 1.f / total;
+      const int row = tile * RT + n, i = row / a.group, head = hk * a.group + row % a.group;
+      char* out = a.o + b * a.os_b + (int64_t)(r.row0 + i) * a.os_n + head * a.os_h;
+      *reinterpret_cast<uint32_t*>(out + 4 * tid) = narrow<BF>(x[0] * inv) | (uint32_t)narrow<BF>(x[1] * inv) << 16;
+      if (a.lse && tid == 0)
+        a.lse[b * a.ls_b + (int64_t)(r.row0 + i) * a.ls_n + head * a.ls_h] = M == -INFINITY ? M : M + logf(total);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The tile kernel: requests of many rows (prompts, chunks of them), bound by the
+// matrix cores. A tile is 256 packed rows, 8 waves x 32. Two groups of four
+// waves, one wave of each on a SIMD, run a phase apart: a wave alternates an
+// MFMA step (S^T(j) = K(j) Q^T interleaved with O^T += V^T(j-1) P^T(j-1)) with a
+// softmax step (S(j) into P(j)), so that on every SIMD one wave feeds the matrix
+// pipe while the other does its softmax; the phases are separated by barriers. LDS
+// holds two K and two V blocks of 128 keys, 256-byte rows placed as in the row
+// kernel. During its softmax of block j group 1 loads K(j + 2) and V(j + 1)
+// into the slots that were read last in the MFMA steps before; their page numbers
+// were fetched (scalar loads) a step earlier.
+//
+// The blocks that every row of the tile sees whole come first, in a loop without
+// mask code, then the others: the order of keys is free in the online softmax.
+//
+// With fewer tiles than CUs (a chunk behind a long cache) the lists of blocks are
+// cut into parts, a workgroup each, joined by a merge kernel. The lengths are
+// known on the GPU alone, so it decides there.
+constexpr int TT = 256;                     // rows of a tile
+constexpr int TTHREADS = 512;
+constexpr int TBLOCK = BLOCK * ROW_BYTES;   // bytes of a K or V block
+constexpr int kTileLds = 4 * TBLOCK;
+constexpr int kTileItems = 512;             // parts of a launch that cuts tiles, at most
+constexpr int kTileGroups = 256;            // parts it aims at
+constexpr int kMinPart = 4;                 // blocks of a part, at least
+
+template <bool PAGED>
+__device__ __forceinline__ int tile_count(const AttnArgs& a, const Request& r) {
+  const int64_t rows = (int64_t)r.n * a.group;
+  return rows > a.rows_max ? (int)((rows + TT - 1) / TT) : 0;
+}
+// At least the blocks of any tile of the request.
+__device__ __forceinline__ int tile_blocks(const AttnArgs& a, const Request& r) {
+  const Blocks all = blocks(a, r, r.pos, r.pos + r.n - 1);
+  const int span = min(TT / a.group + 2, r.n);
+  const int64_t near = ((int64_t)a.window + span + BLOCK - 1) / BLOCK + 1 + (a.sinks + BLOCK - 1) / BLOCK;
+  return max((int)min((int64_t)all.total(), near), 1);
+}
+
+// What a workgroup of the tile kernel does: a part of a tile's blocks.
+struct Item {
+  int b, hk, tile, part, parts, length;     // length: blocks of a part
+  int index, tile_index;                    // place among all parts, all tiles
+};
+
+template <bool BF, bool PAGED>
+__device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, char* lds, int* flag) {
+  int tid;
+  asm volatile("v_mov_b32 %0, %1" : "=v"(tid) : "v"((int)threadIdx.x));
+  const int lane = tid & 63, l32 = lane & 31, hf = lane >> 5, lr = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int grp = wave >> 2, dw = wave & 3;
+  const Request r = uniform_request<PAGED>(a, it.b);
+  const int b = it.b, hk = it.hk;
+  const int rows = r.n * a.group;
+  const int row0 = it.tile * TT + wave * 32;
+  const int row = min(row0 + l32, rows - 1);
+  const bool row_ok = row0 + l32 < rows;
+  const int i = row / a.group, head = hk * a.group + row % a.group;
+  const int pos = r.pos + i;
+  const int tile_last = min(it.tile * TT + TT, rows) - 1;
+  const Blocks bl = uniform(blocks(a, r, uniform(r.pos + it.tile * TT / a.group), uniform(r.pos + tile_last / a.group)));
+  // The list: whole blocks, then those with the mask in order.
+  const int nfull_all = bl.f1 - bl.f0;
+  auto list = [&](int s) {
+    int x = s - nfull_all;
+    if (x < 0) return bl.f0 + s;
+    if (x < bl.ns) return x;
+    x += bl.w0 - bl.ns;
+    return x < bl.f0 ? x : x + nfull_all;
+  };
+  const int total = bl.total();
+  const int s0 = min(it.part * it.length, total);
+  const int nblk = min(it.length, total - s0);        // of this part
+  const int nfull = min(max(nfull_all - s0, 0), nblk);
+  const bool part = it.parts > 1;
+  auto block_at = [&](int s) { return list(s0 + s); };
+
+  const int64_t orow = b * a.os_b + (int64_t)(r.row0 + i) * a.os_n + head * a.os_h;
+  const int64_t lrow = b * a.ls_b + (int64_t)(r.row0 + i) * a.ls_n + head * a.ls_h;
+  float* const prow = a.topart + ((int64_t)it.index * TT + wave * 32 + l32) * HD;
+  float* const plse = a.tlpart + (int64_t)it.index * TT + wave * 32 + l32;
+  if (nblk <= 0) {                          // uniform: no row sees a key of this part
+    const float bad = r.bad ? NAN : 0.f;
+    if (!row_ok) return;
+    if (part) {
+      if (hf == 0) *plse = r.bad ? NAN : -INFINITY;
+      return;                               // the merge reads no O of weight 0
+    }
+    u16x8 z;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[e] = narrow<BF>(bad);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) *reinterpret_cast<u16x8*>(a.o + orow + (2 * x + hf) * 16) = z;
+    if (a.lse && hf == 0) a.lse[lrow] = r.bad ? NAN : -INFINITY;
+    return;
+  }
+
+  const Stream<PAGED> st(a, r, b, hk);
+  const char* qrow = a.q + b * a.qs_b + (int64_t)(r.row0 + i) * a.qs_n + head * a.qs_h;
+  h8 qf[8];
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) qf[kk] = *reinterpret_cast<const h8*>(qrow + (kk * 2 + hf) * 16);
+
+  // Loads: instruction x of group 1's wave dw fills rows 16x + 4dw .. + 3 of a block, one
+  // of the 16-key groups.
+  const int koff = (4 * dw + lr) * st.ks_n + ((lane & 15) ^ (4 * dw + lr)) * 16;
+  const int voff = (4 * dw + lr) * st.vs_n + ((lane & 15) ^ (4 * lr)) * 16;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+  bool bad = r.bad;
+  int kid[8], vid[8], nid[8];
+  int kkey = 0, vkey = 0, nkey = 0;         // first keys of the blocks whose pages these are
+  auto fetch = [&](int s) {
+    nkey = s < nblk ? block_at(s) * BLOCK : 1 << 30;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) nid[x] = st.page(nkey + 16 * x);
+  };
+  auto shift_ids = [&]() {
+    vkey = kkey;
+    kkey = nkey;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      vid[x] = kid[x];
+      kid[x] = nid[x];
+    }
+  };
+  auto load_k = [&](int x, int slot) {
+    bad |= st.missing(kkey + 16 * x, kid[x]);
+    dma_to_lds(st.k_rsrc(kkey + 16 * x, kid[x]), lds0 + slot * TBLOCK + (4 * x + dw) * 1024, koff, 0);
+  };
+  auto load_v = [&](int x, int slot) {
+    dma_to_lds(st.v_rsrc(vkey + 16 * x, vid[x]), lds0 + (2 + slot) * TBLOCK + (4 * x + dw) * 1024, voff, 0);
+  };
+
+  f32x16 acc[4], s[4];
+  h8 p[8];
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt) acc[dt] = f32x16{};
+  float m = -INFINITY, l = 0.f;
+
+  // Operands: K row 32t + l32, chunk 2kk + hf; V as described at Fragments.
+  const int k_lane = l32 * ROW_BYTES + ((hf ^ (l32 & 15)) << 4);
+  int v_lane[4];
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt) {
+    const int e = (lane & 15) >> 2;
+    v_lane[dt] = (4 * hf + e) * ROW_BYTES + (4 * (dt ^ e) + 2 * (lr & 1) + ((lane & 3) >> 1)) * 16 + (lane & 1) * 8;
+  }
+  // Operand x of a step: even x QK product n = x / 2 (score tile n % 4, k-step n / 4),
+  // odd x PV product n (O tile n % 4, 16-key step n / 4), so consecutive
+  // products of a kind go to different accumulators.
+  constexpr int BOTH = 0, QK = 1, PV = 2, PF = 4;
+  auto ld = [&](const char* kb, const char* vb, int x) -> h8 {
+    const int n = x >> 1;
+    if ((x & 1) == 0)
+      return *reinterpret_cast<const h8*>(kb + (k_lane ^ ((n / 4) << 5)) + (n % 4) * 32 * ROW_BYTES);
+    const char* at = vb + v_lane[n % 4] + (n / 4) * 16 * ROW_BYTES;
+    return __builtin_shufflevector(lds_read_tr(at), lds_read_tr(at + 8 * ROW_BYTES), 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  h8 fr[PF];
+  auto operand = [](int kind, int x) constexpr { return kind == BOTH ? x : 2 * x + (kind == PV); };
+  auto preload = [&](const char* kb, const char* vb, auto kind) {
+#pragma unroll
+    for (int x = 0; x < PF; ++x) fr[x] = ld(kb, vb, operand(decltype(kind)::value, x));
+  };
+  auto mfma_step = [&](const char* kb, const char* vb, auto preloaded, auto kind) {
+    constexpr int KIND = decltype(kind)::value;
+    constexpr int N = KIND == BOTH ? 64 : 32;
+    if constexpr (!decltype(preloaded)::value) preload(kb, vb, kind);
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+      const h8 f = fr[x % PF];
+      const int op = operand(KIND, x), n = op >> 1;
+      if ((op & 1) == 0)
+        s[n % 4] = mma<BF>(f, qf[n / 4], n < 4 ? f32x16{} : s[n % 4]);
+      else
+        acc[n % 4] = mma<BF>(f, p[n / 4], acc[n % 4]);
+      if (x + PF < N) fr[x % PF] = ld(kb, vb, operand(KIND, x + PF));
+      __builtin_amdgcn_sched_barrier(0);    // operand reads stay PF products ahead
+    }
+  };
+  auto softmax = [&](int j, auto with_mask, auto&& at) {
+    if constexpr (decltype(with_mask)::value) {
+      const int base = block_at(j) * BLOCK + 4 * hf;
+      const int hi = min(pos, r.keys - 1) - base, lo = pos - a.window + 1 - base, sink = a.sinks - base;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) s[t][x] = masked(s[t][x], 32 * t + 8 * (x >> 2) + (x & 3), hi, lo, sink);
+    }
+    softmax_step<BF, 4>(s, p, m, l, acc, a.c, at);
+  };
+  const std::integral_constant<bool, false> loads, whole;
+  const std::integral_constant<bool, true> preloaded, with_mask;
+  const std::integral_constant<int, BOTH> both;
+  const std::integral_constant<int, QK> qk;
+  const std::integral_constant<int, PV> pv;
+  auto kslot = [&](int j) { return lds + (j & 1) * TBLOCK; };
+  auto vslot = [&](int j) { return lds + (2 + (j & 1)) * TBLOCK; };
+
+  // Phase 2j + grp is a wave's MFMA step for block j, phase 2j + grp + 1 its
+  // softmax; all waves pass the same 2 nblk + 3 barriers. K(j) and V(j) are in
+  // slots j % 2. Group 1 loads K(0) before the first barrier, K(1) and V(0) in
+  // phase 0 and K(j + 2), V(j + 1) in phase 2j + 2, and waits for them at the
+  // end of the next phase, before the barrier that publishes them.
+  if (tid == 0) *flag = 0;
+  const bool idle = row0 >= rows;           // this wave has no row: it loads and waits only
+  if (grp == 1) {
+    fetch(0);
+    shift_ids();
+#pragma unroll
+    for (int x = 0; x < 8; ++x) load_k(x, 0);
+    fetch(1);
+    shift_ids();
+    wait_loads<0>();
+  }
+  // The compiler waits for its own loads here, before the key loop.
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) asm volatile("" ::"v"(qf[kk]));
+  lds_barrier();
+  if (grp == 0) {
+    if (idle) {
+      for (int j = 0; j < 2 * nblk + 2; ++j) lds_barrier();
+    } else {
+      auto step = [&](int j, auto kind, auto mask) {
+        mfma_step(kslot(j), vslot(j + 1), loads, kind);
+        lds_barrier();
+        softmax(j, mask, [](int) {});
+        lds_barrier();
+      };
+      if (nfull > 0)
+        step(0, qk, whole);
+      else
+        step(0, qk, with_mask);
+      int j = 1;
+      for (; j < nfull; ++j) step(j, both, whole);
+      for (; j < nblk; ++j) step(j, both, with_mask);
+      mfma_step(kslot(nblk), vslot(nblk + 1), loads, pv);
+      lds_barrier();
+      lds_barrier();
+    }
+  } else {
+    // Phase 0: the loads of K(1) and V(0).
+#pragma unroll
+    for (int x = 0; x < 8; ++x) load_k(x, 1);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) load_v(x, 0);
+    fetch(2);
+    shift_ids();
+    if (idle) {
+      lds_barrier();
+      for (int j = 0; j < nblk; ++j) {
+        wait_loads<0>();
+        lds_barrier();
+        fetch(j + 3);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) load_k(x, j & 1);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) load_v(x, (j + 1) & 1);
+        shift_ids();
+        lds_barrier();
+      }
+      wait_loads<0>();
+      lds_barrier();
+    } else {
+      preload(kslot(0), vslot(0), qk);
+      lds_barrier();
+      auto step = [&](int j, auto kind, auto mask) {
+        mfma_step(kslot(j), vslot(j + 1), preloaded, kind);
+        wait_loads<0>();
+        lds_barrier();
+        fetch(j + 3);
+        // 16 loads over the 32 pairs of exponentials.
+        softmax(j, mask, [&](int x) {
+          if (x & 1) return;
+          __builtin_amdgcn_sched_barrier(0);
+          if (x < 16)
+            load_k(x / 2, j & 1);
+          else
+            load_v(x / 2 - 8, (j + 1) & 1);
+          __builtin_amdgcn_sched_barrier(0);
+        });
+        shift_ids();
+        preload(kslot(j + 1), vslot(j), both);
+        lds_barrier();
+      };
+      if (nfull > 0)
+        step(0, qk, whole);
+      else
+        step(0, qk, with_mask);
+      int j = 1;
+      for (; j < nfull; ++j) step(j, both, whole);
+      for (; j < nblk; ++j) step(j, both, with_mask);
+      mfma_step(kslot(nblk), vslot(nblk + 1), loads, pv);
+      wait_loads<0>();
+      lds_barrier();
+    }
+    if (bad && lane == 0) *flag = 1;
+  }
+  lds_barrier();                            // nobody reads the ring any more; flag is set
+  const bool poisoned = *flag != 0 || r.bad;
+
+  // Results. l is 0 for a row that saw no key.
+  float lsum = half_sum(l);
+  if (poisoned) lsum = NAN;
+  const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+  const float lse = (__builtin_amdgcn_logf(lsum) + m * a.c) * LN2;
+  float check = 0.f;
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int x = 0; x < 16; ++x) check += acc[dt][x] * 0.f;
+  const bool sick = row_ok && is_nan(check) && !is_nan(lsum);
+  uint64_t again = nfull < nblk ? __builtin_amdgcn_ballot_w64(sick) : 0;
+  again |= again >> 32;
+  again &= 0xffffffffull;                   // a bit a row
+  const uint32_t repaired = (uint32_t)again;
+  while (again) {
+    const int n = __ffsll((unsigned long long)again) - 1;
+    again &= again - 1;
+    const int rr = row0 + n, ri = rr / a.group, rh = hk * a.group + rr % a.group;
+    float x[2], rl;
+    repair_row<BF, PAGED>(a, st, a.q + b * a.qs_b + (int64_t)(r.row0 + ri) * a.qs_n + rh * a.qs_h, r.pos + ri, 0, nblk,
+                          block_at, x, rl);
+    if (part) {
+      float* dst = a.topart + ((int64_t)it.index * TT + wave * 32 + n) * HD;
+      dst[2 * lane] = x[0];
+      dst[2 * lane + 1] = x[1];
+      if (lane == 0) a.tlpart[(int64_t)it.index * TT + wave * 32 + n] = rl;
+    } else {
+      char* dst = a.o + b * a.os_b + (int64_t)(r.row0 + ri) * a.os_n + rh * a.os_h;
+      *reinterpret_cast<uint32_t*>(dst + 4 * lane) = narrow<BF>(x[0]) | (uint32_t)narrow<BF>(x[1]) << 16;
+      if (a.lse && lane == 0) a.lse[b * a.ls_b + (int64_t)(r.row0 + ri) * a.ls_n + rh * a.ls_h] = rl;
+    }
+  }
+  const bool done = repaired >> l32 & 1;
+  if (part) {
+    if (!row_ok || done) return;
+    if (hf == 0) *plse = lse;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<float4*>(prow + dt * 32 + 8 * g + 4 * hf) =
+            float4{acc[dt][4 * g] * inv, acc[dt][4 * g + 1] * inv, acc[dt][4 * g + 2] * inv, acc[dt][4 * g + 3] * inv};
+    return;
+  }
+  if (a.lse && hf == 0 && row_ok && !done) a.lse[lrow] = lse;
+  // A lane holds 4 dims here and there of one row; the wave turns its rows around
+  // in 8 KiB of the ring, chunk c of row n at c ^ n % 16, and stores whole rows.
+  char* turn = lds + wave * (32 * ROW_BYTES);
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      u16x4 out;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[e] = narrow<BF>(acc[dt][4 * g + e] * inv);
+      *reinterpret_cast<u16x4*>(turn + l32 * ROW_BYTES + (((4 * dt + g) ^ (l32 & 15)) << 4) + hf * 8) = out;
+    }
+#pragma unroll
+  for (int x = 0; x < 8; ++x) {
+    const int n = 4 * x + lr;
+    const u32x4 val = *reinterpret_cast<const u32x4*>(turn + n * ROW_BYTES + (((lane & 15) ^ (n & 15)) << 4));
+    const int64_t dst = (int64_t)(uint32_t)__shfl((int)orow, n) | (int64_t)__shfl((int)(orow >> 32), n) << 32;
+    if (row0 + n < rows && !(repaired >> n & 1)) *reinterpret_cast<u32x4*>(a.o + dst + (lane & 15) * 16) = val;
+  }
+}
+
+// Which item a workgroup has. The 8 dies take workgroups in turn (die = workgroup
+// % 8), and the tiles that read the same keys should be on one die at a time, so
+// that its L2 fetches them once, while every die gets its share of long and short
+// tiles. With h = gcd(8, KV heads), die x takes the KV heads hk = x mod h and, of
+// request b's tiles counted from the last (the longest come first), those with
+// number (x / h + b) mod (8 / h).
+template <bool BF, bool PAGED>
+__global__ void __launch_bounds__(TTHREADS) __attribute__((amdgpu_waves_per_eu(2, 2)))
+fa_serve_tiles_kernel(AttnArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ uint64_t wave_sum[TTHREADS / 64][4];
+  __shared__ int found[8];
+  __shared__ int flag;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int die = blockIdx.x & 7, slot0 = blockIdx.x >> 3;
+  const int h = min(a.heads_kv & -a.heads_kv, 8), step = 8 / h;
+  const int per = (a.batch + TTHREADS - 1) / TTHREADS;
+  const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
+  auto wave_scan = [&](uint64_t v) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint64_t other = __shfl_up(v, d);
+      if (lane >= d) v += other;
+    }
+    return v;
+  };
+  // Blocks and tiles of all requests, for the length of a part.
+  uint64_t blocks_all = 0, tiles_mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    const Request r = request<PAGED>(a, b);
+    const uint64_t t = (uint64_t)a.heads_kv * tile_count<PAGED>(a, r);
+    if (t) blocks_all += t * tile_blocks(a, r);
+    tiles_mine += t;
+  }
+  const uint64_t scan_b = wave_scan(blocks_all), scan_t = wave_scan(tiles_mine);
+  if (lane == 63) {
+    wave_sum[wave][0] = scan_b;
+    wave_sum[wave][1] = scan_t;
+  }
+  if (tid < 8) found[tid] = -1;
+  __syncthreads();
+  uint64_t total_b = 0, total_t = 0, tiles_before = scan_t - tiles_mine;
+#pragma unroll
+  for (int w = 0; w < TTHREADS / 64; ++w) {
+    if (w < wave) tiles_before += wave_sum[w][1];
+    total_b += wave_sum[w][0];
+    total_t += wave_sum[w][1];
+  }
+  total_b = uniform(total_b);
+  // Cut if there are fewer tiles than CUs: then there are at most kTileGroups
+  // parts and one more a tile.
+  const bool split = a.split && uniform(total_t) < kTileGroups;
+  if (a.split && blockIdx.x == 0 && tid == 0) a.tdesc[0] = split ? (int)total_t : 0;
+  const int length = split ? uniform(max((int)((total_b + kTileGroups - 1) / kTileGroups), kMinPart)) : 1 << 30;
+  auto parts_of = [&](const Request& r) { return split ? (tile_blocks(a, r) + length - 1) / length : 1; };
+  // Tiles of request b that die `die` takes: those numbered x, x + step, ..
+  auto first_of = [&](int b) { return (die / h + b) % step; };
+  auto tiles_of = [&](int b, int tiles) { return max(0, (tiles - first_of(b) + step - 1) / step); };
+  uint64_t mine = 0, parts_mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    const Request r = request<PAGED>(a, b);
+    const int tiles = tile_count<PAGED>(a, r);
+    if (!tiles) continue;
+    const int parts = parts_of(r);
+    mine += (uint64_t)(a.heads_kv / h) * tiles_of(b, tiles) * parts;
+    parts_mine += (uint64_t)a.heads_kv * tiles * parts;
+  }
+  const uint64_t scan_m = wave_scan(mine), scan_p = wave_scan(parts_mine);
+  if (lane == 63) {
+    wave_sum[wave][2] = scan_m;
+    wave_sum[wave][3] = scan_p;
+  }
+  __syncthreads();
+  uint64_t before = scan_m - mine, total = 0, parts_before = scan_p - parts_mine;
+#pragma unroll
+  for (int w = 0; w < TTHREADS / 64; ++w) {
+    if (w < wave) {
+      before += wave_sum[w][2];
+      parts_before += wave_sum[w][3];
+    }
+    total += wave_sum[w][2];
+  }
+  for (uint64_t x = slot0; x < total; x += gridDim.x >> 3) {
+    __syncthreads();                        // found[] and the ring are free
+    if (before <= x && x < before + mine) {
+      uint64_t at = before, t_at = tiles_before, p_at = parts_before;
+      for (int b = b0;; ++b) {
+        const Request r = request<PAGED>(a, b);
+        const int tiles = tile_count<PAGED>(a, r);
+        if (!tiles) continue;
+        const int parts = parts_of(r), here = tiles_of(b, tiles);
+        const uint64_t n = (uint64_t)(a.heads_kv / h) * here * parts;
+        if (x >= at + n) {
+          at += n;
+          t_at += (uint64_t)a.heads_kv * tiles;
+          p_at += (uint64_t)a.heads_kv * tiles * parts;
+          continue;
+        }
+        // Tiles of one head and part consecutive.
+        const int rel = (int)(x - at), unit = rel / here;
+        const int part = unit % parts, hk = unit / parts * h + die % h;
+        const int tile = tiles - 1 - (first_of(b) + rel % here * step);
+        found[0] = b;
+        found[1] = hk;
+        found[2] = tile;
+        found[3] = part;
+        found[4] = parts;
+        found[5] = (int)(p_at + ((uint64_t)hk * tiles + tile) * parts + part);
+        found[6] = (int)(t_at + (uint64_t)hk * tiles + tile);
+        break;
+      }
+    }
+    __syncthreads();
+    Item it;
+    it.b = uniform(found[0]);
+    it.hk = uniform(found[1]);
+    it.tile = uniform(found[2]);
+    it.part = uniform(found[3]);
+    it.parts = uniform(found[4]);
+    it.index = uniform(found[5]);
+    it.tile_index = uniform(found[6]);
+    it.length = length;
+    if (split && it.part == 0 && tid == 0) {
+      int* d = a.tdesc + (it.tile_index + 1) * DESC_INTS;
+      d[0] = it.b;
+      d[1] = it.hk;
+      d[2] = it.tile;
+      d[3] = it.index;
+      d[4] = it.parts;
+    }
+    tile_item<BF, PAGED>(a, it, lds, &flag);
+  }
+}
+
+// Joins the parts of the tiles, 8 rows a workgroup, 32 lanes a row (4 dims each).
+template <bool BF, bool PAGED>
+__global__ void __launch_bounds__(256) fa_serve_tiles_merge_kernel(AttnArgs a) {
+  const int t = blockIdx.x >> 5;
+  if (t >= a.tdesc[0]) return;
+  const int* d = a.tdesc + (t + 1) * DESC_INTS;
+  const int parts = d[4];
+  if (parts < 2) return;
+  const int b = d[0], hk = d[1], n = (blockIdx.x & 31) * 8 + (threadIdx.x >> 5), dim = (threadIdx.x & 31) * 4;
+  const Request r = request<PAGED>(a, b);
+  const int row = d[2] * TT + n;
+  if (row >= r.n * a.group) return;
+  const int64_t at = (int64_t)d[3] * TT + n;
+  float M = -INFINITY;
+  for (int s = 0; s < parts; ++s) M = smax(M, a.tlpart[at + (int64_t)s * TT]);
+  float total = 0.f;
+  float4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < parts; ++s) {
+    const float x = a.tlpart[at + (int64_t)s * TT];
+    const float4 v = *reinterpret_cast<const float4*>(a.topart + (at + (int64_t)s * TT) * HD + dim);
+    if (x == -INFINITY) continue;           // such a part has written no O
+    const float w = expf(x - M);
+    total += w;
+    o.x = __builtin_fmaf(w, v.x, o.x);
+    o.y = __builtin_fmaf(w, v.y, o.y);
+    o.z = __builtin_fmaf(w, v.z, o.z);
+    o.w = __builtin_fmaf(w, v.w, o.w);
+  }
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  const int i = row / a.group, head = hk * a.group + row % a.group;
+  const u16x4 val = {narrow<BF>(o.x * inv), narrow<BF>(o.y * inv), narrow<BF>(o.z * inv), narrow<BF>(o.w * inv)};
+  *reinterpret_cast<u16x4*>(a.o + b * a.os_b + (int64_t)(r.row0 + i) * a.os_n + head * a.os_h + dim * 2) = val;
+  if (a.lse && dim == 0)
+    a.lse[b * a.ls_b + (int64_t)(r.row0 + i) * a.ls_n + head * a.ls_h] = M == -INFINITY ? M : M + logf(total);
+}
+
+// ---------------------------------------------------------------------------
+// Host side.
+
+// A request's packed rows up to this many go to the row kernel.
+constexpr int64_t kRowsMax = 64;
+
+struct Kernels {
+  const void *rows, *rows_merge, *tiles, *tiles_merge;
+};
+template <bool BF, bool PAGED>
+constexpr Kernels kernels_of() {
+  return {reinterpret_cast<const void*>(&fa_serve_rows_kernel<BF, PAGED>),
+          reinterpret_cast<const void*>(&fa_serve_rows_merge_kernel<BF, PAGED>),
+          reinterpret_cast<const void*>(&fa_serve_tiles_kernel<BF, PAGED>),
+          reinterpret_cast<const void*>(&fa_serve_tiles_merge_kernel<BF, PAGED>)};
+}
+const Kernels kKernels[2][2] = {{kernels_of<false, false>(), kernels_of<false, true>()},
+                                {kernels_of<true, false>(), kernels_of<true, true>()}};
+
+// Raises the LDS limit of every attention kernel on the current device, once.
+constexpr int kMaxDevices = 64;
+int ensure_lds_limits() {
+  static std::atomic<bool> done[kMaxDevices];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return FA_SERVE_ERR_LAUNCH;
+  const bool known = dev >= 0 && dev < kMaxDevices;
+  if (known && done[dev].load(std::memory_order_acquire)) return FA_SERVE_OK;
+  for (const auto& type : kKernels)
+    for (const Kernels& k : type) {
+      if (hipFuncSetAttribute(k.rows, hipFuncAttributeMaxDynamicSharedMemorySize, kRowsLds) != hipSuccess ||
+          hipFuncSetAttribute(k.tiles, hipFuncAttributeMaxDynamicSharedMemorySize, kTileLds) != hipSuccess)
+        return FA_SERVE_ERR_LAUNCH;
+    }
+  if (known) done[dev].store(true, std::memory_order_release);
+  return FA_SERVE_OK;
+}
+
+// What a call launches, from what the host knows: bounds on the rows.
+struct LaunchPlan {
+  bool rows = false, tiles = false, split = false;
+  int rows_max = 0;                         // for the kernels: see AttnArgs
+  int64_t tiles_max = 0;                    // tiles, if the requests are all consistent
+  uint64_t opart = 0, lpart = 0, desc = 0, topart = 0, tlpart = 0, tdesc = 0, end = 0;   // offsets
+};
+LaunchPlan launch_plan(int64_t batch, int64_t heads_kv, int64_t group, int64_t tokens, int64_t max_new, bool even) {
+  LaunchPlan p;
+  p.rows_max = (int)kRowsMax;
+  p.tiles = max_new * group > kRowsMax;
+  // One kernel takes every request if all have few rows, or all as many, or
+  // there is one request.
+  p.rows = !p.tiles || (batch > 1 && !even);
+  if (!p.rows) p.rows_max = 0;
+  if (!p.tiles) p.rows_max = INT32_MAX;
+  p.tiles_max = heads_kv * (even ? batch * ((max_new * group + TT - 1) / TT) : tokens * group / TT + batch);
+  p.split = p.tiles && (!even || p.tiles_max < kTileGroups);
+  auto take = [&](uint64_t bytes) {
+    const uint64_t at = p.end;
+    p.end += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  if (p.rows) {
+    p.opart = take((uint64_t)2 * kRowsGroups * RT * HD * 4);
+    p.lpart = take((uint64_t)2 * kRowsGroups * RT * 4);
+    p.desc = take((uint64_t)kRowsGroups * DESC_INTS * 4);
+  }
+  if (p.split) {
+    p.topart = take((uint64_t)kTileItems * TT * HD * 4);
+    p.tlpart = take((uint64_t)kTileItems * TT * 4);
+    p.tdesc = take((uint64_t)(kTileGroups + 1) * DESC_INTS * 4);
+  }
+  return p;
+}
+
+int check_heads(int64_t heads_q, int64_t heads_kv) {
+  return heads_q < 1 || heads_kv < 1 || heads_q > 4096 || heads_q % heads_kv ? FA_SERVE_ERR_GEOMETRY : FA_SERVE_OK;
+}
+int check_mask(int64_t window, int64_t sinks) {
+  return window < 0 || sinks < 0 || (sinks && !window) ? FA_SERVE_ERR_WINDOW : FA_SERVE_OK;
+}
+// c = scale log2 e: scores times c must neither vanish nor overflow for ordinary scores.
+int check_scale(float scale) { return scale > 0.f && isfinite(scale) ? FA_SERVE_OK : FA_SERVE_ERR_SCALE; }
+int check_type(int32_t type) {
+  return type == FA_SERVE_FP16 || type == FA_SERVE_BF16 ? FA_SERVE_OK : FA_SERVE_ERR_TYPE;
+}
+// Rows of K and V within a page (or of a contiguous tensor) are 32-bit apart.
+int check_rows(int64_t stride) { return stride < HD || stride >= 1 << 25 ? FA_SERVE_ERR_STRIDE : FA_SERVE_OK; }
+
+int run(const AttnArgs& filled, const LaunchPlan& lp, int32_t type, bool paged, void* workspace, void* stream) {
+  AttnArgs a = filled;
+  int rc = check_stream_device(stream);
+  if (!rc) rc = ensure_lds_limits();
+  if (rc) return rc;
+  char* ws = static_cast<char*>(workspace);
+  a.opart = reinterpret_cast<float*>(ws + lp.opart);
+  a.lpart = reinterpret_cast<float*>(ws + lp.lpart);
+  a.desc = reinterpret_cast<int*>(ws + lp.desc);
+  a.topart = reinterpret_cast<float*>(ws + lp.topart);
+  a.tlpart = reinterpret_cast<float*>(ws + lp.tlpart);
+  a.tdesc = reinterpret_cast<int*>(ws + lp.tdesc);
+  a.rows_max = lp.rows_max;
+  a.split = lp.split;
+  a.groups = kRowsGroups;
+  const Kernels& k = kKernels[type == FA_SERVE_BF16][paged];
+  void* args[] = {&a};
+  if (lp.tiles) {
+    // A workgroup for every item there can be, a multiple of 8 (each die's
+    // share rounds up once a request and head); they loop, so any number is right.
+    const int64_t h = std::min<int64_t>(a.heads_kv & -(int64_t)a.heads_kv, 8);
+    int64_t grid = 8 * (lp.tiles_max / 8 + a.heads_kv / h * a.batch + 1);
+    grid = std::min<int64_t>(std::max<int64_t>(grid, lp.split ? kTileItems : 8), 1 << 20);
+    rc = enqueue(k.tiles, dim3((unsigned)grid), dim3(TTHREADS), args, kTileLds, stream);
+    if (!rc && lp.split) rc = enqueue(k.tiles_merge, dim3(kTileGroups * 32), dim3(256), args, 0, stream);
+  }
+  if (!rc && lp.rows) {
+    rc = enqueue(k.rows, dim3(kRowsGroups), dim3(RTHREADS), args, kRowsLds, stream);
+    if (!rc) rc = enqueue(k.rows_merge, dim3(kRowsGroups - 1), dim3(256), args, 0, stream);
+  }
+  return rc;
+}
+
+// The row kernel counts the key blocks of all its items in 32 bits.
+int check_work(const LaunchPlan& lp, int64_t batch, int64_t heads_kv, int64_t group, int64_t rows, int64_t keys) {
+  if (!lp.rows) return FA_SERVE_OK;
+  const int64_t tiles = lp.tiles ? batch * (kRowsMax / RT) : rows * group / RT + batch;
+  return tiles <= ((int64_t)1 << 31) / heads_kv / (keys / BLOCK + 2) ? FA_SERVE_OK : FA_SERVE_ERR_GEOMETRY;
+}
+
+int check_paged(const fa_paged* p, LaunchPlan* lp) {
+  if (!p) return FA_SERVE_ERR_NULL;
+  const int64_t limit = (int64_t)1 << 30;
+  int rc = check_heads(p->heads_q, p->heads_kv);
+  if (rc) return rc;
+  if (p->batch < 1 || p->batch > 4096 || p->tokens < 0 || p->max_new < 1 || p->pages < 0 || p->pages > limit ||
+      p->max_pages < 1 || p->max_pages > limit)
+    return FA_SERVE_ERR_GEOMETRY;
+  if (page_shift(p->page_size) < 0) return FA_SERVE_ERR_PAGE;
+  // Rows and keys are counted in 32 bits, packed rows too.
+  if (p->tokens >= limit / (p->heads_q / p->heads_kv) || p->max_pages > limit / p->page_size)
+    return FA_SERVE_ERR_GEOMETRY;
+  rc = check_type(p->type);
+  if (!rc) rc = check_mask(p->window, p->sinks);
+  if (!rc) rc = check_scale(p->scale);
+  if (rc) return rc;
+  *lp = launch_plan(p->batch, p->heads_kv, p->heads_q / p->heads_kv, p->tokens,
+                    std::min(p->max_new, std::max<int64_t>(p->tokens, 1)), false);
+  return check_work(*lp, p->batch, p->heads_kv, p->heads_q / p->heads_kv, p->tokens, p->max_pages * p->page_size);
+}
+
+int check_window(const fa_window* p, LaunchPlan* lp) {
+  if (!p) return FA_SERVE_ERR_NULL;
+  const int64_t limit = (int64_t)1 << 30;
+  int rc = check_heads(p->heads_q, p->heads_kv);
+  if (rc) return rc;
+  if (p->batch < 1 || p->batch > 65536 || p->seq_q < 1 || p->seq_k < 1 || p->seq_k >= limit ||
+      p->seq_q >= limit / (p->heads_q / p->heads_kv))
+    return FA_SERVE_ERR_GEOMETRY;
+  rc = check_type(p->type);
+  if (!rc && (p->window < 1 || p->sinks < 0)) rc = FA_SERVE_ERR_WINDOW;
+  if (!rc) rc = check_scale(p->scale);
+  if (!rc && p->causal != FA_WINDOW_TOP_LEFT && p->causal != FA_WINDOW_BOTTOM_RIGHT) rc = FA_SERVE_ERR_CAUSAL;
+  if (rc) return rc;
+  *lp = launch_plan(p->batch, p->heads_kv, p->heads_q / p->heads_kv, p->batch * p->seq_q, p->seq_q, true);
+  return check_work(*lp, p->batch, p->heads_kv, p->heads_q / p->heads_kv, p->batch * p->seq_q, p->seq_k);
+}
+
+AttnArgs mask_args(int64_t window, int64_t sinks, float scale) {
+  AttnArgs a{};
+  a.window = window ? (int)std::min<int64_t>(window, NO_WINDOW) : NO_WINDOW;
+  a.sinks = (int)std::min<int64_t>(sinks, NO_WINDOW);
+  a.c = (float)((double)scale * LOG2E);
+  return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fa_paged_workspace_bytes(const fa_paged* p, uint64_t* bytes) {
+  LaunchPlan lp;
+  const int rc = check_paged(p, &lp);
+  if (rc) return rc;
+  if (!bytes) return FA_SERVE_ERR_NULL;
+  *bytes = lp.end;
+  return FA_SERVE_OK;
+}
+
+int fa_paged_fwd(const fa_paged* p, const void* q, const void* k_cache, const void* v_cache, const int32_t* table,
+                 const int32_t* starts, const int32_t* lengths, void* o, float* lse, void* workspace,
+                 uint64_t workspace_bytes, void* stream) {
+  LaunchPlan lp;
+  int rc = check_paged(p, &lp);
+  if (rc) return rc;
+  if (p->table_stride < p->max_pages || p->table_stride > (int64_t)1 << 30) return FA_SERVE_ERR_STRIDE;
+  for (const int64_t* s : {p->q, p->o})
+    if (!rc) rc = check_strides(s, 2);
+  for (const int64_t* s : {p->k_cache, p->v_cache}) {
+    if (!rc) rc = check_strides(s, 3);
+    if (!rc) rc = check_rows(s[1]);
+    // The page's byte stride is a 32-bit factor of a 64-bit product.
+    if (!rc && s[0] >= (int64_t)1 << 31) rc = FA_SERVE_ERR_STRIDE;
+  }
+  if (rc) return rc;
+  if (!k_cache || !v_cache || !table || !starts || !lengths || (p->tokens && (!q || !o))) return FA_SERVE_ERR_NULL;
+  for (const void* ptr : {q, k_cache, v_cache, (const void*)o, (const void*)workspace})
+    if (!aligned(ptr, 16)) return FA_SERVE_ERR_ALIGN;
+  for (const void* ptr : {(const void*)table, (const void*)starts, (const void*)lengths, (const void*)lse})
+    if (!aligned(ptr, 4)) return FA_SERVE_ERR_ALIGN;
+  if ((lp.end && !workspace) || workspace_bytes < lp.end) return FA_SERVE_ERR_WORKSPACE;
+  if (p->tokens == 0) return FA_SERVE_OK;
+  AttnArgs a = mask_args(p->window, p->sinks, p->scale);
+  a.q = static_cast<const char*>(q);
+  a.k = static_cast<const char*>(k_cache);
+  a.v = static_cast<const char*>(v_cache);
+  a.o = static_cast<char*>(o);
+  a.lse = lse;
+  a.table = table;
+  a.starts = starts;
+  a.lengths = lengths;
+  a.table_stride = p->table_stride;
+  a.qs_n = 2 * p->q[0];
+  a.qs_h = 2 * p->q[1];
+  a.os_n = 2 * p->o[0];
+  a.os_h = 2 * p->o[1];
+  a.ks_b = 2 * p->k_cache[0];
+  a.ks_n = (int)(2 * p->k_cache[1]);
+  a.ks_h = 2 * p->k_cache[2];
+  a.vs_b = 2 * p->v_cache[0];
+  a.vs_n = (int)(2 * p->v_cache[1]);
+  a.vs_h = 2 * p->v_cache[2];
+  a.ls_n = p->heads_q;
+  a.ls_h = 1;
+  a.batch = (int)p->batch;
+  a.heads_kv = (int)p->heads_kv;
+  a.group = (int)(p->heads_q / p->heads_kv);
+  a.tokens = (int)p->tokens;
+  a.pages = (int)p->pages;
+  a.shift = page_shift(p->page_size);
+  a.max_pages = (int)p->max_pages;
+  return run(a, lp, p->type, true, workspace, stream);
+}
+
+int fa_window_workspace_bytes(const fa_window* p, uint64_t* bytes) {
+  LaunchPlan lp;
+  const int rc = check_window(p, &lp);
+  if (rc) return rc;
+  if (!bytes) return FA_SERVE_ERR_NULL;
+  *bytes = lp.end;
+  return FA_SERVE_OK;
+}
+
+int fa_window_fwd(const fa_window* p, const void* q, const void* k, const void* v, void* o, float* lse,
+                  void* workspace, uint64_t workspace_bytes, void* stream) {
+  LaunchPlan lp;
+  int rc = check_window(p, &lp);
+  if (rc) return rc;
+  for (const int64_t* s : {p->q, p->k, p->v, p->o})
+    if (!rc) rc = check_strides(s, 3);
+  if (!rc) rc = check_rows(p->k[2]);
+  if (!rc) rc = check_rows(p->v[2]);
+  if (rc) return rc;
+  if (!q || !k || !v || !o) return FA_SERVE_ERR_NULL;
+  for (const void* ptr : {q, k, v, (const void*)o, (const void*)workspace})
+    if (!aligned(ptr, 16)) return FA_SERVE_ERR_ALIGN;
+  if (!aligned(lse, 4)) return FA_SERVE_ERR_ALIGN;
+  if ((lp.end && !workspace) || workspace_bytes < lp.end) return FA_SERVE_ERR_WORKSPACE;
+  AttnArgs a = mask_args(p->window, p->sinks, p->scale);
+  a.q = static_cast<const char*>(q);
+  a.k = static_cast<const char*>(k);
+  a.v = static_cast<const char*>(v);
+  a.o = static_cast<char*>(o);
+  a.lse = lse;
+  a.qs_b = 2 * p->q[0];
+  a.qs_h = 2 * p->q[1];
+  a.qs_n = 2 * p->q[2];
+  a.os_b = 2 * p->o[0];
+  a.os_h = 2 * p->o[1];
+  a.os_n = 2 * p->o[2];
+  a.ks_b = 2 * p->k[0];
+  a.ks_h = 2 * p->k[1];
+  a.ks_n = (int)(2 * p->k[2]);
+  a.vs_b = 2 * p->v[0];
+  a.vs_h = 2 * p->v[1];
+  a.vs_n = (int)(2 * p->v[2]);
+  a.ls_b = p->heads_q * p->seq_q;
+  a.ls_h = p->seq_q;
+  a.ls_n = 1;
+  a.batch = (int)p->batch;
+  a.heads_kv = (int)p->heads_kv;
+  a.group = (int)(p->heads_q / p->heads_kv);
+  a.seq_q = (int)p->seq_q;
+  a.seq_k = (int)p->seq_k;
+  a.off = p->causal == FA_WINDOW_BOTTOM_RIGHT ? (int)(p->seq_k - p->seq_q) : 0;
+  return run(a, lp, p->type, false, workspace, stream);
+}
+
+const char* fa_serve_strerror(int status) {
+  switch (status) {
+    case FA_SERVE_OK: return "ok";
+    case FA_SERVE_ERR_NULL: return "a required pointer is NULL";
+    case FA_SERVE_ERR_GEOMETRY: return "a size is out of range, or heads_q is no multiple of heads_kv";
+    case FA_SERVE_ERR_TYPE: return "unknown element type";
+    case FA_SERVE_ERR_PAGE: return "page size must be a power of two from 16 to 65536";
+    case FA_SERVE_ERR_ALIGN: return "a pointer or stride is not aligned";
+    case FA_SERVE_ERR_WORKSPACE: return "workspace missing or too small";
+    case FA_SERVE_ERR_WINDOW: return "invalid window or sinks";
+    case FA_SERVE_ERR_SCALE: return "scale must be finite and positive";
+    case FA_SERVE_ERR_ROTARY: return "rotary dims must be a multiple of 16 from 16 to 128, in a known layout";
+    case FA_SERVE_ERR_LAUNCH: return "the HIP runtime rejected a launch";
+    case FA_SERVE_ERR_STRIDE: return "a stride is out of range";
+    case FA_SERVE_ERR_CAUSAL: return "unknown causal alignment";
+    case FA_SERVE_ERR_DEVICE: return "the stream belongs to another device than the current one";
+    default: return "unknown status";
+  }
+}
+
+}  // extern "C"
