@@ -80,6 +80,16 @@ struct AttnArgs {
   int groups;                               // workgroups of the row kernel
 };
 
+// The kernel's arguments through an address that the compiler cannot follow: read
+// again where they are needed instead of staying in scalar registers (or spilling)
+// across a key loop.
+typedef const AttnArgs __attribute__((address_space(4))) ConstArgs;
+__device__ __forceinline__ ConstArgs& fresh_args() {
+  uint64_t addr = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());
+  asm volatile("" : "+s"(addr));
+  return *reinterpret_cast<ConstArgs*>(addr);
+}
+
 // A value every lane of the wave has, in a scalar register (integer divisions, for
 // one, are made in vector registers).
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -284,7 +294,7 @@ struct Stream {
   // The page of the group at `key` (for a group past the last key, of that key).
   __device__ __forceinline__ int page(int key) const {
     if constexpr (PAGED)
-      return __builtin_amdgcn_readfirstlane(table[max(min(key, keys - 1), 0) >> shift]);
+      return table[max(min(key, keys - 1), 0) >> shift];
     else
       return 0;
   }
@@ -320,8 +330,8 @@ struct Stream {
 // 2 lane, 2 lane + 1) and lse of the keys it sees, which alone are read. The
 // whole wave works on one row; for the rare rows that NaN in a hidden key's V
 // has reached.
-template <bool BF, bool PAGED, typename BlockAt>
-__device__ __forceinline__ void repair_row(const AttnArgs& a, const Stream<PAGED>& st, const char* qrow, int pos,
+template <bool BF, bool PAGED, typename Args, typename BlockAt>
+__device__ __forceinline__ void repair_row(const Args& a, const Stream<PAGED>& st, const char* qrow, int pos,
                                            int s0, int s1, BlockAt&& block_at, float (&o)[2], float& lse) {
   const int lane = threadIdx.x & 63;
   const uint32_t qw = *reinterpret_cast<const uint32_t*>(qrow + 4 * lane);
@@ -457,8 +467,8 @@ __device__ __forceinline__ void row_item(const AttnArgs& a, const Request& r, in
     }
   };
   auto pages_of = [&](int key, int (&id)[2]) {
-    id[0] = st.page(key);
-    id[1] = st.page(key + 16);
+    id[0] = uniform(st.page(key));
+    id[1] = uniform(st.page(key + 16));
   };
 
   const char* qrow = a.q + b * a.qs_b + (int64_t)(r.row0 + i) * a.qs_n + head * a.qs_h;
@@ -707,74 +717,127 @@ fa_serve_rows_kernel(AttnArgs a) {
 
 // Joins the pieces of the items that several workgroups share:
 //   O = sum w_s O_s / sum w_s, w_s = exp(lse_s - M), M = max lse_s, lse = M + ln sum w_s.
-// Workgroup g > 0 whose share starts inside an item is one of the K that do; the
-// j-th of them takes rows j, j + K, .. of the item's 32, so a launch's joins are
-// spread evenly however many pieces an item has. A row's pieces are read by 8
-// groups of 32 lanes, 4 dims a lane, and joined in LDS.
+// Workgroup g > 0 whose share starts inside an item is one of the K = pieces - 1 that
+// do, and they share its join, so that a launch's joins are spread evenly however
+// many pieces an item has. Up to kFewPieces pieces, 32 lanes take a row (4 dims each),
+// 8 rows at once; beyond, the workgroup takes a quarter of a row's dims at a
+// time, 32 groups of 8 lanes reading a 32nd of the pieces each.
+// Both forms have as many loads in flight as there are pieces to a lane: the first
+// form alone took 23.6 us for one row's 512 pieces (131072 keys), a workgroup a row
+// 16.6 us for 8 rows of 2 or 3 (64 requests).
+constexpr int kFewPieces = 32;
 template <bool BF, bool PAGED>
 __global__ void __launch_bounds__(256) fa_serve_rows_merge_kernel(AttnArgs a) {
   __shared__ float weight[kRowsGroups];
-  __shared__ float red[8][HD];
+  __shared__ float red[32][36];             // padded: 8 rows of 4 lanes' dims at a time
   __shared__ float wave_red[4];
   const int* desc = a.desc + (blockIdx.x + 1) * DESC_INTS;
   const int first = desc[3];
   if (first < 0) return;
   const int b = desc[0], hk = desc[1], tile = desc[2], last = desc[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int boundaries = last - first, pieces = boundaries + 1;
+  const int boundaries = last - first, pieces = boundaries + 1, mine = (int)blockIdx.x - first;
   const Request r = request<PAGED>(a, b);
   const int rows = min(r.n * a.group - tile * RT, RT);
   auto piece = [&](int s) { return (int64_t)(2 * (first + s) + (s == 0)); };
-  for (int n = (int)blockIdx.x - first; n < rows; n += boundaries) {
-    float mine = -INFINITY;
-    for (int s = tid; s < pieces; s += 256) mine = smax(mine, a.lpart[piece(s) * RT + n]);
+  auto row_of = [&](int n, int& i, int& head) {
+    const int row = tile * RT + n;
+    i = row / a.group;
+    head = hk * a.group + row % a.group;
+  };
+  auto out_row = [&](int n) {
+    int i, head;
+    row_of(n, i, head);
+    return a.o + b * a.os_b + (int64_t)(r.row0 + i) * a.os_n + head * a.os_h;
+  };
+  auto out_lse = [&](int n, float M, float total) {
+    if (!a.lse) return;
+    int i, head;
+    row_of(n, i, head);
+    a.lse[b * a.ls_b + (int64_t)(r.row0 + i) * a.ls_n + head * a.ls_h] = M == -INFINITY ? M : M + logf(total);
+  };
+  if (pieces <= kFewPieces) {
+    const int l32 = tid & 31;
+    for (int n = mine + (tid >> 5) * boundaries; n < rows; n += 8 * boundaries) {
+      const float x = l32 < pieces ? a.lpart[piece(l32) * RT + n] : -INFINITY;
+      float M = x;
 #pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) mine = smax(mine, __shfl_xor(mine, d));
-    __syncthreads();                        // the last row's LDS has been read
-    if (lane == 0) wave_red[wave] = mine;
-    __syncthreads();
-    const float M = smax(smax(wave_red[0], wave_red[1]), smax(wave_red[2], wave_red[3]));
-    __syncthreads();
-    float total = 0.f;
-    for (int s = tid; s < pieces; s += 256) {
-      const float x = a.lpart[piece(s) * RT + n];
+      for (int d = 16; d >= 1; d >>= 1) M = smax(M, __shfl_xor(M, d, 32));
       const float w = x == -INFINITY ? 0.f : expf(x - M);
-      weight[s] = w;
+      float total = w;
+#pragma unroll
+      for (int d = 16; d >= 1; d >>= 1) total += __shfl_xor(total, d, 32);
+      float4 o = {0.f, 0.f, 0.f, 0.f};
+      for (int s0 = 0; s0 < pieces; s0 += 8) {
+        float4 v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)         // past the last piece: that one again, weight 0
+          v[e] = *reinterpret_cast<const float4*>(a.opart + (piece(min(s0 + e, pieces - 1)) * RT + n) * HD + 4 * l32);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float ws = __shfl(w, min(s0 + e, 31), 32) * (s0 + e < pieces ? 1.f : 0.f);
+          o.x = __builtin_fmaf(ws, v[e].x, o.x);
+          o.y = __builtin_fmaf(ws, v[e].y, o.y);
+          o.z = __builtin_fmaf(ws, v[e].z, o.z);
+          o.w = __builtin_fmaf(ws, v[e].w, o.w);
+        }
+      }
+      const float inv = total == 0.f ? 0.f : 1.f / total;
+      *reinterpret_cast<u16x4*>(out_row(n) + 8 * l32) =
+          u16x4{narrow<BF>(o.x * inv), narrow<BF>(o.y * inv), narrow<BF>(o.z * inv), narrow<BF>(o.w * inv)};
+      if (l32 == 0) out_lse(n, M, total);
+    }
+    return;
+  }
+  for (int u = mine; u < 4 * rows; u += boundaries) {
+    const int n = u >> 2, dim = (u & 3) * 32 + (tid & 7) * 4, grp = tid >> 3;
+    float x[kRowsGroups / 256], M = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kRowsGroups / 256; ++k) {
+      const int s = tid + 256 * k;
+      x[k] = s < pieces ? a.lpart[piece(s) * RT + n] : -INFINITY;
+      M = smax(M, x[k]);
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) M = smax(M, __shfl_xor(M, d));
+    __syncthreads();                        // the last unit's LDS has been read
+    if (lane == 0) wave_red[wave] = M;
+    __syncthreads();
+    M = smax(smax(wave_red[0], wave_red[1]), smax(wave_red[2], wave_red[3]));
+    float total = 0.f;
+#pragma unroll
+    for (int k = 0; k < kRowsGroups / 256; ++k) {
+      const float w = x[k] == -INFINITY ? 0.f : expf(x[k] - M);
+      weight[tid + 256 * k] = w;
       total += w;
     }
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) total += __shfl_xor(total, d);
-    if (lane == 0) wave_red[wave] = total;
     __syncthreads();
-    total = (wave_red[0] + wave_red[1]) + (wave_red[2] + wave_red[3]);
-    const int grp = tid >> 5, dim = (tid & 31) * 4;
+    if (lane == 0) wave_red[wave] = total;
     float4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int s = grp; s < pieces; s += 8) {
-      const float w = weight[s];
-      const float4 v = *reinterpret_cast<const float4*>(a.opart + (piece(s) * RT + n) * HD + dim);
-      if (w != 0.f) {                       // a piece without keys may hold NaN
+#pragma unroll
+    for (int k = 0; k < kRowsGroups / 32; ++k) {
+      const int s = grp + 32 * k;
+      if (s < pieces) {
+        const float4 v = *reinterpret_cast<const float4*>(a.opart + (piece(s) * RT + n) * HD + dim);
+        const float w = weight[s];
         o.x = __builtin_fmaf(w, v.x, o.x);
         o.y = __builtin_fmaf(w, v.y, o.y);
         o.z = __builtin_fmaf(w, v.z, o.z);
         o.w = __builtin_fmaf(w, v.w, o.w);
       }
     }
-    *reinterpret_cast<float4*>(&red[grp][dim]) = o;
+    *reinterpret_cast<float4*>(&red[grp][(tid & 7) * 4]) = o;
     __syncthreads();
-    if (tid < 64) {
-      float x[2] = {0.f, 0.f};
+    if (tid < 32) {
+      total = (wave_red[0] + wave_red[1]) + (wave_red[2] + wave_red[3]);
+      float sum = 0.f;
 #pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        x[0] += red[s][2 * tid];
-        x[1] += red[s][2 * tid + 1];
-      }
+      for (int s = 0; s < 32; ++s) sum += red[s][tid];
       const float inv = total == 0.f ? 0.f : 1.f / total;
-      const int row = tile * RT + n, i = row / a.group, head = hk * a.group + row % a.group;
-      char* out = a.o + b * a.os_b + (int64_t)(r.row0 + i) * a.os_n + head * a.os_h;
-      *reinterpret_cast<uint32_t*>(out + 4 * tid) = narrow<BF>(x[0] * inv) | (uint32_t)narrow<BF>(x[1] * inv) << 16;
-      if (a.lse && tid == 0)
-        a.lse[b * a.ls_b + (int64_t)(r.row0 + i) * a.ls_n + head * a.ls_h] = M == -INFINITY ? M : M + logf(total);
+      reinterpret_cast<uint16_t*>(out_row(n))[(u & 3) * 32 + tid] = narrow<BF>(sum * inv);
+      if ((u & 3) == 0 && tid == 0) out_lse(n, M, total);
     }
   }
 }
@@ -802,8 +865,12 @@ constexpr int TTHREADS = 512;
 constexpr int TBLOCK = BLOCK * ROW_BYTES;   // bytes of a K or V block
 constexpr int kTileLds = 4 * TBLOCK;
 constexpr int kTileItems = 512;             // parts of a launch that cuts tiles, at most
-constexpr int kTileGroups = 256;            // parts it aims at
-constexpr int kMinPart = 4;                 // blocks of a part, at least
+constexpr int kTileGroups = 256;            // CUs: launches of fewer tiles may cut them
+constexpr int kCuts = 24;                   // parts of the longest tile, at most
+// Costs in units of a key block (3.5 us on a CU): what an item takes besides its
+// blocks if it is a whole tile, or a part (256 rows of FP32 O to write), a merge
+// kernel, and every part's share of it (128 KiB to read).
+constexpr float kWholeCost = 2.f, kPartCost = 5.f, kMergeCost = 2.f, kMergeShare = 0.014f;
 
 template <bool PAGED>
 __device__ __forceinline__ int tile_count(const AttnArgs& a, const Request& r) {
@@ -837,7 +904,9 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
   const int row0 = it.tile * TT + wave * 32;
   const int row = min(row0 + l32, rows - 1);
   const bool row_ok = row0 + l32 < rows;
-  const int i = row / a.group, head = hk * a.group + row % a.group;
+  const int group = a.group, window = a.window, sinks = a.sinks;
+  const float c = a.c;
+  const int i = row / group, head = hk * group + row % group;
   const int pos = r.pos + i;
   const int tile_last = min(it.tile * TT + TT, rows) - 1;
   const Blocks bl = uniform(blocks(a, r, uniform(r.pos + it.tile * TT / a.group), uniform(r.pos + tile_last / a.group)));
@@ -857,23 +926,20 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
   const bool part = it.parts > 1;
   auto block_at = [&](int s) { return list(s0 + s); };
 
-  const int64_t orow = b * a.os_b + (int64_t)(r.row0 + i) * a.os_n + head * a.os_h;
-  const int64_t lrow = b * a.ls_b + (int64_t)(r.row0 + i) * a.ls_n + head * a.ls_h;
-  float* const prow = a.topart + ((int64_t)it.index * TT + wave * 32 + l32) * HD;
-  float* const plse = a.tlpart + (int64_t)it.index * TT + wave * 32 + l32;
   if (nblk <= 0) {                          // uniform: no row sees a key of this part
     const float bad = r.bad ? NAN : 0.f;
     if (!row_ok) return;
-    if (part) {
-      if (hf == 0) *plse = r.bad ? NAN : -INFINITY;
-      return;                               // the merge reads no O of weight 0
+    if (part) {                             // the merge reads no O of weight 0
+      if (hf == 0) a.tlpart[(int64_t)it.index * TT + wave * 32 + l32] = r.bad ? NAN : -INFINITY;
+      return;
     }
     u16x8 z;
 #pragma unroll
     for (int e = 0; e < 8; ++e) z[e] = narrow<BF>(bad);
+    char* out = a.o + b * a.os_b + (int64_t)(r.row0 + i) * a.os_n + head * a.os_h;
 #pragma unroll
-    for (int x = 0; x < 8; ++x) *reinterpret_cast<u16x8*>(a.o + orow + (2 * x + hf) * 16) = z;
-    if (a.lse && hf == 0) a.lse[lrow] = r.bad ? NAN : -INFINITY;
+    for (int x = 0; x < 8; ++x) *reinterpret_cast<u16x8*>(out + (2 * x + hf) * 16) = z;
+    if (a.lse && hf == 0) a.lse[b * a.ls_b + (int64_t)(r.row0 + i) * a.ls_n + head * a.ls_h] = r.bad ? NAN : -INFINITY;
     return;
   }
 
@@ -889,28 +955,28 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
   const int voff = (4 * dw + lr) * st.vs_n + ((lane & 15) ^ (4 * lr)) * 16;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
   bool bad = r.bad;
-  int kid[8], vid[8], nid[8];
-  int kkey = 0, vkey = 0, nkey = 0;         // first keys of the blocks whose pages these are
+  // Pages of the next K block to load, of the V block to load beside it and of the
+  // K block after: lane x holds that of the block's 16-key group x % 8.
+  int kid = 0, vid = 0, nid = 0;
+  int kkey = 0, vkey = 0, nkey = 0;         // first keys of those blocks
   auto fetch = [&](int s) {
     nkey = s < nblk ? block_at(s) * BLOCK : 1 << 30;
-#pragma unroll
-    for (int x = 0; x < 8; ++x) nid[x] = st.page(nkey + 16 * x);
+    nid = st.page(nkey + 16 * (lane & 7));
   };
   auto shift_ids = [&]() {
     vkey = kkey;
     kkey = nkey;
-#pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      vid[x] = kid[x];
-      kid[x] = nid[x];
-    }
+    vid = kid;
+    kid = nid;
   };
   auto load_k = [&](int x, int slot) {
-    bad |= st.missing(kkey + 16 * x, kid[x]);
-    dma_to_lds(st.k_rsrc(kkey + 16 * x, kid[x]), lds0 + slot * TBLOCK + (4 * x + dw) * 1024, koff, 0);
+    const int id = __builtin_amdgcn_readlane(kid, x);
+    bad |= st.missing(kkey + 16 * x, id);
+    dma_to_lds(st.k_rsrc(kkey + 16 * x, id), lds0 + slot * TBLOCK + (4 * x + dw) * 1024, koff, 0);
   };
   auto load_v = [&](int x, int slot) {
-    dma_to_lds(st.v_rsrc(vkey + 16 * x, vid[x]), lds0 + (2 + slot) * TBLOCK + (4 * x + dw) * 1024, voff, 0);
+    const int id = __builtin_amdgcn_readlane(vid, x);
+    dma_to_lds(st.v_rsrc(vkey + 16 * x, id), lds0 + (2 + slot) * TBLOCK + (4 * x + dw) * 1024, voff, 0);
   };
 
   f32x16 acc[4], s[4];
@@ -963,13 +1029,13 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
   auto softmax = [&](int j, auto with_mask, auto&& at) {
     if constexpr (decltype(with_mask)::value) {
       const int base = block_at(j) * BLOCK + 4 * hf;
-      const int hi = min(pos, r.keys - 1) - base, lo = pos - a.window + 1 - base, sink = a.sinks - base;
+      const int hi = min(pos, r.keys - 1) - base, lo = pos - window + 1 - base, sink = sinks - base;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int x = 0; x < 16; ++x) s[t][x] = masked(s[t][x], 32 * t + 8 * (x >> 2) + (x & 3), hi, lo, sink);
     }
-    softmax_step<BF, 4>(s, p, m, l, acc, a.c, at);
+    softmax_step<BF, 4>(s, p, m, l, acc, c, at);
   };
   const std::integral_constant<bool, false> loads, whole;
   const std::integral_constant<bool, true> preloaded, with_mask;
@@ -1082,10 +1148,11 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
   const bool poisoned = *flag != 0 || r.bad;
 
   // Results. l is 0 for a row that saw no key.
+  ConstArgs& f = fresh_args();
   float lsum = half_sum(l);
   if (poisoned) lsum = NAN;
   const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
-  const float lse = (__builtin_amdgcn_logf(lsum) + m * a.c) * LN2;
+  const float lse = (__builtin_amdgcn_logf(lsum) + m * f.c) * LN2;
   float check = 0.f;
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt)
@@ -1099,25 +1166,27 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
   while (again) {
     const int n = __ffsll((unsigned long long)again) - 1;
     again &= again - 1;
-    const int rr = row0 + n, ri = rr / a.group, rh = hk * a.group + rr % a.group;
+    const int rr = row0 + n, ri = rr / f.group, rh = hk * f.group + rr % f.group;
     float x[2], rl;
-    repair_row<BF, PAGED>(a, st, a.q + b * a.qs_b + (int64_t)(r.row0 + ri) * a.qs_n + rh * a.qs_h, r.pos + ri, 0, nblk,
+    repair_row<BF, PAGED>(f, st, f.q + b * f.qs_b + (int64_t)(r.row0 + ri) * f.qs_n + rh * f.qs_h, r.pos + ri, 0, nblk,
                           block_at, x, rl);
     if (part) {
-      float* dst = a.topart + ((int64_t)it.index * TT + wave * 32 + n) * HD;
+      float* dst = f.topart + ((int64_t)it.index * TT + wave * 32 + n) * HD;
       dst[2 * lane] = x[0];
       dst[2 * lane + 1] = x[1];
-      if (lane == 0) a.tlpart[(int64_t)it.index * TT + wave * 32 + n] = rl;
+      if (lane == 0) f.tlpart[(int64_t)it.index * TT + wave * 32 + n] = rl;
     } else {
-      char* dst = a.o + b * a.os_b + (int64_t)(r.row0 + ri) * a.os_n + rh * a.os_h;
+      char* dst = f.o + b * f.os_b + (int64_t)(r.row0 + ri) * f.os_n + rh * f.os_h;
       *reinterpret_cast<uint32_t*>(dst + 4 * lane) = narrow<BF>(x[0]) | (uint32_t)narrow<BF>(x[1]) << 16;
-      if (a.lse && lane == 0) a.lse[b * a.ls_b + (int64_t)(r.row0 + ri) * a.ls_n + rh * a.ls_h] = rl;
+      if (f.lse && lane == 0) f.lse[b * f.ls_b + (int64_t)(r.row0 + ri) * f.ls_n + rh * f.ls_h] = rl;
     }
   }
   const bool done = repaired >> l32 & 1;
+  const int orow = min(row0 + l32, rows - 1), oi = orow / f.group, ohead = hk * f.group + orow % f.group;
   if (part) {
     if (!row_ok || done) return;
-    if (hf == 0) *plse = lse;
+    if (hf == 0) f.tlpart[(int64_t)it.index * TT + wave * 32 + l32] = lse;
+    float* const prow = f.topart + ((int64_t)it.index * TT + wave * 32 + l32) * HD;
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
@@ -1126,9 +1195,10 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
             float4{acc[dt][4 * g] * inv, acc[dt][4 * g + 1] * inv, acc[dt][4 * g + 2] * inv, acc[dt][4 * g + 3] * inv};
     return;
   }
-  if (a.lse && hf == 0 && row_ok && !done) a.lse[lrow] = lse;
+  if (f.lse && hf == 0 && row_ok && !done) f.lse[b * f.ls_b + (int64_t)(r.row0 + oi) * f.ls_n + ohead * f.ls_h] = lse;
   // A lane holds 4 dims here and there of one row; the wave turns its rows around
   // in 8 KiB of the ring, chunk c of row n at c ^ n % 16, and stores whole rows.
+  const int64_t obase = b * f.os_b + (int64_t)(r.row0 + oi) * f.os_n + ohead * f.os_h;
   char* turn = lds + wave * (32 * ROW_BYTES);
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt)
@@ -1143,22 +1213,24 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
   for (int x = 0; x < 8; ++x) {
     const int n = 4 * x + lr;
     const u32x4 val = *reinterpret_cast<const u32x4*>(turn + n * ROW_BYTES + (((lane & 15) ^ (n & 15)) << 4));
-    const int64_t dst = (int64_t)(uint32_t)__shfl((int)orow, n) | (int64_t)__shfl((int)(orow >> 32), n) << 32;
-    if (row0 + n < rows && !(repaired >> n & 1)) *reinterpret_cast<u32x4*>(a.o + dst + (lane & 15) * 16) = val;
+    const int64_t dst = (int64_t)(uint32_t)__shfl((int)obase, n) | (int64_t)__shfl((int)(obase >> 32), n) << 32;
+    if (row0 + n < rows && !(repaired >> n & 1)) *reinterpret_cast<u32x4*>(f.o + dst + (lane & 15) * 16) = val;
   }
 }
 
 // Which item a workgroup has. The 8 dies take workgroups in turn (die = workgroup
 // % 8), and the tiles that read the same keys should be on one die at a time, so
 // that its L2 fetches them once, while every die gets its share of long and short
-// tiles. With h = gcd(8, KV heads), die x takes the KV heads hk = x mod h and, of
-// request b's tiles counted from the last (the longest come first), those with
-// number (x / h + b) mod (8 / h).
+// tiles. Whole tiles: with h = gcd(8, KV heads), die x takes the KV heads hk = x mod h
+// and, of request b's tiles counted from the last (the longest come first), those
+// with number (x / h + b) mod (8 / h). Parts: the tiles of a part are consecutive,
+// and each die has an eighth of all parts, consecutive ones.
 template <bool BF, bool PAGED>
 __global__ void __launch_bounds__(TTHREADS) __attribute__((amdgpu_waves_per_eu(2, 2)))
 fa_serve_tiles_kernel(AttnArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  __shared__ uint64_t wave_sum[TTHREADS / 64][4];
+  __shared__ uint64_t wave_sum[TTHREADS / 64][5];
+  __shared__ float cut_cost[kCuts];
   __shared__ int found[8];
   __shared__ int flag;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -1174,20 +1246,26 @@ fa_serve_tiles_kernel(AttnArgs a) {
     }
     return v;
   };
-  // Blocks and tiles of all requests, for the length of a part.
-  uint64_t blocks_all = 0, tiles_mine = 0;
+  // Tiles and blocks of all requests and the longest tile's.
+  uint64_t tiles_mine = 0, blocks_mine = 0;
+  int longest = 0;
+  int2* const loads = reinterpret_cast<int2*>(lds);   // of every request: tiles, blocks
   for (int b = b0; b < b1; ++b) {
     const Request r = request<PAGED>(a, b);
-    const uint64_t t = (uint64_t)a.heads_kv * tile_count<PAGED>(a, r);
-    if (t) blocks_all += t * tile_blocks(a, r);
+    const int t = a.heads_kv * tile_count<PAGED>(a, r), n = t ? tile_blocks(a, r) : 0;
+    if (a.split) loads[b] = int2{t, n};
     tiles_mine += t;
+    blocks_mine += (uint64_t)t * n;
+    longest = max(longest, n);
   }
-  const uint64_t scan_b = wave_scan(blocks_all), scan_t = wave_scan(tiles_mine);
+  const uint64_t scan_b = wave_scan(blocks_mine), scan_t = wave_scan(tiles_mine);
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) longest = max(longest, __shfl_xor(longest, d));
   if (lane == 63) {
     wave_sum[wave][0] = scan_b;
     wave_sum[wave][1] = scan_t;
+    wave_sum[wave][2] = longest;
   }
-  if (tid < 8) found[tid] = -1;
   __syncthreads();
   uint64_t total_b = 0, total_t = 0, tiles_before = scan_t - tiles_mine;
 #pragma unroll
@@ -1195,91 +1273,106 @@ fa_serve_tiles_kernel(AttnArgs a) {
     if (w < wave) tiles_before += wave_sum[w][1];
     total_b += wave_sum[w][0];
     total_t += wave_sum[w][1];
+    longest = max(longest, (int)wave_sum[w][2]);
   }
-  total_b = uniform(total_b);
-  // Cut if there are fewer tiles than CUs: then there are at most kTileGroups
-  // parts and one more a tile.
-  const bool split = a.split && uniform(total_t) < kTileGroups;
+  // Cut if there are fewer tiles than CUs and that is modelled to be faster: with
+  // parts of at most `length` blocks, a round of parts for every 256 of them. Wave w
+  // looks at cuts of the longest tile into w + 1, w + 9, .. parts.
+  int length = 1 << 30;
+  if (a.split && total_t < kTileGroups) {   // uniform
+    for (int p = wave + 1; p <= kCuts; p += TTHREADS / 64) {
+      const int n = max((longest + p - 1) / p, 1);
+      int items = 0;
+      for (int b = lane; b < a.batch; b += 64) items += loads[b].x * ((loads[b].y + n - 1) / n);
+#pragma unroll
+      for (int d = 32; d >= 1; d >>= 1) items += __shfl_xor(items, d);
+      const float rounds = (float)((items + kTileGroups - 1) / kTileGroups);
+      // Uncut tiles of different lengths share the one round there is.
+      const float cost = p == 1 ? longest + kWholeCost
+                                : rounds * (n + kPartCost) + kMergeCost + kMergeShare * items;
+      if (lane == 0) cut_cost[p - 1] = items <= kTileItems ? cost : INFINITY;
+    }
+    __syncthreads();
+    int best = 1;
+    for (int p = 2; p <= kCuts; ++p)
+      if (cut_cost[p - 1] < cut_cost[best - 1]) best = p;
+    if (best > 1) length = uniform(max((longest + best - 1) / best, 1));
+  }
+  const bool split = length < 1 << 30;
   if (a.split && blockIdx.x == 0 && tid == 0) a.tdesc[0] = split ? (int)total_t : 0;
-  const int length = split ? uniform(max((int)((total_b + kTileGroups - 1) / kTileGroups), kMinPart)) : 1 << 30;
   auto parts_of = [&](const Request& r) { return split ? (tile_blocks(a, r) + length - 1) / length : 1; };
-  // Tiles of request b that die `die` takes: those numbered x, x + step, ..
+  // Of whole tiles, those of request b that die `die` takes.
   auto first_of = [&](int b) { return (die / h + b) % step; };
   auto tiles_of = [&](int b, int tiles) { return max(0, (tiles - first_of(b) + step - 1) / step); };
-  uint64_t mine = 0, parts_mine = 0;
+  auto items_of = [&](int b, int tiles, int parts) {
+    return split ? a.heads_kv * tiles * parts : a.heads_kv / h * tiles_of(b, tiles);
+  };
+  uint64_t mine = 0;
   for (int b = b0; b < b1; ++b) {
     const Request r = request<PAGED>(a, b);
     const int tiles = tile_count<PAGED>(a, r);
-    if (!tiles) continue;
-    const int parts = parts_of(r);
-    mine += (uint64_t)(a.heads_kv / h) * tiles_of(b, tiles) * parts;
-    parts_mine += (uint64_t)a.heads_kv * tiles * parts;
+    if (tiles) mine += items_of(b, tiles, parts_of(r));
   }
-  const uint64_t scan_m = wave_scan(mine), scan_p = wave_scan(parts_mine);
-  if (lane == 63) {
-    wave_sum[wave][2] = scan_m;
-    wave_sum[wave][3] = scan_p;
-  }
+  const uint64_t scan_m = wave_scan(mine);
+  if (lane == 63) wave_sum[wave][3] = scan_m;
   __syncthreads();
-  uint64_t before = scan_m - mine, total = 0, parts_before = scan_p - parts_mine;
+  uint64_t before = scan_m - mine, total = 0;
 #pragma unroll
   for (int w = 0; w < TTHREADS / 64; ++w) {
-    if (w < wave) {
-      before += wave_sum[w][2];
-      parts_before += wave_sum[w][3];
-    }
-    total += wave_sum[w][2];
+    if (w < wave) before += wave_sum[w][3];
+    total += wave_sum[w][3];
   }
-  for (uint64_t x = slot0; x < total; x += gridDim.x >> 3) {
-    __syncthreads();                        // found[] and the ring are free
-    if (before <= x && x < before + mine) {
-      uint64_t at = before, t_at = tiles_before, p_at = parts_before;
-      for (int b = b0;; ++b) {
-        const Request r = request<PAGED>(a, b);
-        const int tiles = tile_count<PAGED>(a, r);
-        if (!tiles) continue;
-        const int parts = parts_of(r), here = tiles_of(b, tiles);
-        const uint64_t n = (uint64_t)(a.heads_kv / h) * here * parts;
-        if (x >= at + n) {
-          at += n;
-          t_at += (uint64_t)a.heads_kv * tiles;
-          p_at += (uint64_t)a.heads_kv * tiles * parts;
-          continue;
-        }
-        // Tiles of one head and part consecutive.
-        const int rel = (int)(x - at), unit = rel / here;
-        const int part = unit % parts, hk = unit / parts * h + die % h;
-        const int tile = tiles - 1 - (first_of(b) + rel % here * step);
-        found[0] = b;
-        found[1] = hk;
-        found[2] = tile;
-        found[3] = part;
-        found[4] = parts;
-        found[5] = (int)(p_at + ((uint64_t)hk * tiles + tile) * parts + part);
-        found[6] = (int)(t_at + (uint64_t)hk * tiles + tile);
-        break;
+  uint64_t x = slot0;
+  if (split) {
+    const uint64_t eighth = (total + 7) / 8;
+    x = slot0 < eighth ? die * eighth + slot0 : total;
+  }
+  if (x >= total) return;                   // uniform
+  if (before <= x && x < before + mine) {
+    uint64_t at = before, t_at = tiles_before;
+    for (int b = b0;; ++b) {
+      const Request r = request<PAGED>(a, b);
+      const int tiles = tile_count<PAGED>(a, r);
+      if (!tiles) continue;
+      const int parts = parts_of(r), n = items_of(b, tiles, parts);
+      if (x >= at + n) {
+        at += n;
+        t_at += (uint64_t)a.heads_kv * tiles;
+        continue;
       }
+      const int rel = (int)(x - at), here = split ? tiles : tiles_of(b, tiles), unit = rel / here;
+      const int hk = split ? unit / parts : unit * h + die % h;
+      const int tile = tiles - 1 - (split ? rel % here : first_of(b) + rel % here * step);
+      const int part = split ? unit % parts : 0;
+      found[0] = b;
+      found[1] = hk;
+      found[2] = tile;
+      found[3] = part;
+      found[4] = parts;
+      found[5] = (int)at + (hk * tiles + tile) * parts + part;
+      found[6] = (int)t_at + hk * tiles + tile;
+      break;
     }
-    __syncthreads();
-    Item it;
-    it.b = uniform(found[0]);
-    it.hk = uniform(found[1]);
-    it.tile = uniform(found[2]);
-    it.part = uniform(found[3]);
-    it.parts = uniform(found[4]);
-    it.index = uniform(found[5]);
-    it.tile_index = uniform(found[6]);
-    it.length = length;
-    if (split && it.part == 0 && tid == 0) {
-      int* d = a.tdesc + (it.tile_index + 1) * DESC_INTS;
-      d[0] = it.b;
-      d[1] = it.hk;
-      d[2] = it.tile;
-      d[3] = it.index;
-      d[4] = it.parts;
-    }
-    tile_item<BF, PAGED>(a, it, lds, &flag);
   }
+  __syncthreads();
+  Item it;
+  it.b = uniform(found[0]);
+  it.hk = uniform(found[1]);
+  it.tile = uniform(found[2]);
+  it.part = uniform(found[3]);
+  it.parts = uniform(found[4]);
+  it.index = uniform(found[5]);
+  it.tile_index = uniform(found[6]);
+  it.length = length;
+  if (split && it.part == 0 && tid == 0) {
+    int* d = a.tdesc + (it.tile_index + 1) * DESC_INTS;
+    d[0] = it.b;
+    d[1] = it.hk;
+    d[2] = it.tile;
+    d[3] = it.index;
+    d[4] = it.parts;
+  }
+  tile_item<BF, PAGED>(a, it, lds, &flag);
 }
 
 // Joins the parts of the tiles, 8 rows a workgroup, 32 lanes a row (4 dims each).
@@ -1424,11 +1517,11 @@ int run(const AttnArgs& filled, const LaunchPlan& lp, int32_t type, bool paged, 
   const Kernels& k = kKernels[type == FA_SERVE_BF16][paged];
   void* args[] = {&a};
   if (lp.tiles) {
-    // A workgroup for every item there can be, a multiple of 8 (each die's
-    // share rounds up once a request and head); they loop, so any number is right.
+    // A workgroup for every item there can be: each die's share of whole tiles
+    // rounds up once a request and head.
     const int64_t h = std::min<int64_t>(a.heads_kv & -(int64_t)a.heads_kv, 8);
     int64_t grid = 8 * (lp.tiles_max / 8 + a.heads_kv / h * a.batch + 1);
-    grid = std::min<int64_t>(std::max<int64_t>(grid, lp.split ? kTileItems : 8), 1 << 20);
+    grid = std::max<int64_t>(grid, lp.split ? kTileItems : 8);
     rc = enqueue(k.tiles, dim3((unsigned)grid), dim3(TTHREADS), args, kTileLds, stream);
     if (!rc && lp.split) rc = enqueue(k.tiles_merge, dim3(kTileGroups * 32), dim3(256), args, 0, stream);
   }
@@ -1439,8 +1532,10 @@ int run(const AttnArgs& filled, const LaunchPlan& lp, int32_t type, bool paged, 
   return rc;
 }
 
-// The row kernel counts the key blocks of all its items in 32 bits.
+// The row kernel counts the key blocks of all its items in 32 bits; the tile
+// kernel's launch has a workgroup a tile.
 int check_work(const LaunchPlan& lp, int64_t batch, int64_t heads_kv, int64_t group, int64_t rows, int64_t keys) {
+  if (lp.tiles && lp.tiles_max + heads_kv * batch >= 1 << 22) return FA_SERVE_ERR_GEOMETRY;
   if (!lp.rows) return FA_SERVE_OK;
   const int64_t tiles = lp.tiles ? batch * (kRowsMax / RT) : rows * group / RT + batch;
   return tiles <= ((int64_t)1 << 31) / heads_kv / (keys / BLOCK + 2) ? FA_SERVE_OK : FA_SERVE_ERR_GEOMETRY;
