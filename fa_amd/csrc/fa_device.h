@@ -87,6 +87,14 @@ __device__ __forceinline__ void dma_to_lds(i32x4 rsrc, uint32_t lds_addr, int vo
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :: "s"(lds_addr), "v"(voff), "s"(rsrc), "s"(soff) : "memory", "m0");
 }
+// dma_to_lds() of a descriptor that a vector instruction may have written just
+// before (v_readfirstlane): a vector-memory instruction may read such a scalar
+// register five wait states later, which the compiler does not see to inside
+// inline assembly.
+__device__ __forceinline__ void dma_to_lds_late(i32x4 rsrc, uint32_t lds_addr, int voff, uint32_t soff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :: "s"(lds_addr), "v"(voff), "s"(rsrc), "s"(soff) : "memory", "m0");
+}
 #pragma clang diagnostic pop
 
 // Workgroup barrier that also drains this wave's outstanding LDS operations,

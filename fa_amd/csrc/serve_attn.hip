@@ -53,6 +53,7 @@ constexpr int BLOCK = 128;                  // keys of a block of the lists belo
 constexpr double LOG2E = 1.4426950408889634;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr int NO_WINDOW = 1 << 30;
+constexpr int kUncut = 1 << 30;
 // The maximum is raised when a score exceeds it by more than this (in powers of
 // two), so P <= 2^8 and O is rescaled rarely.
 constexpr float TAU = 8.f;
@@ -73,6 +74,8 @@ struct AttnArgs {
   float c;
   int rows_max;                             // packed rows of a request that the row kernel takes
   int split;                                // tile kernel: there is room for parts
+  int length;                               // contiguous: blocks of a part (uncut: kUncut)
+  int tile_groups;                          // workgroups of the tile kernel that take tiles
   float *opart, *lpart;                     // row kernel's parts
   int* desc;
   float *topart, *tlpart;                   // tile kernel's parts
@@ -99,6 +102,19 @@ __device__ __forceinline__ uint64_t uniform(uint64_t x) {
          (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
 }
 
+// Sum over this lane and the lanes before it.
+__device__ __forceinline__ uint32_t lanes_sum(uint32_t x) {
+#define ADD_DPP(ctrl, rows) x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, rows, 0xf, false)
+  ADD_DPP(0x111, 0xf);                      // row_shr 1, 2, 4, 8: within 16 lanes
+  ADD_DPP(0x112, 0xf);
+  ADD_DPP(0x114, 0xf);
+  ADD_DPP(0x118, 0xf);
+  ADD_DPP(0x142, 0xa);                      // the last of a row to the next one
+  ADD_DPP(0x143, 0xc);                      // and of the lower to the upper half
+#undef ADD_DPP
+  return x;
+}
+
 // A batch entry: the first of its rows in q, their number, the position of
 // row 0, its keys, and whether its table row is too short for them.
 struct Request {
@@ -106,7 +122,7 @@ struct Request {
   bool bad;
 };
 template <bool PAGED>
-__device__ __forceinline__ Request request(const AttnArgs& a, int b) {
+__host__ __device__ __forceinline__ Request request(const AttnArgs& a, int b) {
   Request r;
   if constexpr (PAGED) {
     const int s0 = min(max(a.starts[b], 0), a.tokens), s1 = min(max(a.starts[b + 1], s0), a.tokens);
@@ -146,9 +162,9 @@ __device__ __forceinline__ Request uniform_request(const AttnArgs& a, int b) {
 // [w0, w1), of which [f0, f1) (within [w0, w1)) are seen whole by every row.
 struct Blocks {
   int ns, w0, w1, f0, f1;
-  __device__ __forceinline__ int total() const { return ns + w1 - w0; }
+  __host__ __device__ __forceinline__ int total() const { return ns + w1 - w0; }
 };
-__device__ __forceinline__ Blocks blocks(const AttnArgs& a, const Request& r, int first, int last) {
+__host__ __device__ __forceinline__ Blocks blocks(const AttnArgs& a, const Request& r, int first, int last) {
   Blocks k;
   const int hi = min(last + 1, r.keys);
   if (hi <= 0) return Blocks{0, 0, 0, 0, 0};
@@ -205,13 +221,28 @@ __device__ __forceinline__ uint16_t narrow(float x) {
     return __builtin_bit_cast(uint16_t, (_Float16)x);
 }
 
-// A score, or -inf for a key outside [.., hi] or outside both [lo, ..] and
-// [.., sink) (all relative to the same key). Sign arithmetic and a bit select:
-// compares and selects would keep a scalar register pair per score alive.
-__device__ __forceinline__ float masked(float s, int key, int hi, int lo, int sink) {
-  const int hidden = min(hi - key, max(key - lo, sink - 1 - key)) >> 31;
-  const uint32_t bits = __float_as_uint(s);
-  return __uint_as_float((bits & ~(uint32_t)hidden) | (0xff800000u & (uint32_t)hidden));
+// Ones in the low n bits, n from anything below 0 to anything above 32.
+__device__ __forceinline__ uint32_t low_bits(int n) {
+  return (uint32_t)(((uint64_t)1 << min(max(n, 0), 32)) - 1);
+}
+// Replaces the scores of the keys a row does not see by -inf: those past hi, and those
+// that are neither from lo on nor before sink, all relative to the lane's first key
+// (register r of 32-key tile t holds key 32t + 8 (r / 4) + r % 4 from there). The
+// keys of a tile become a word of hidden bits, of which each score takes one:
+// two instructions a score. Compares and selects would keep a scalar register
+// pair a score alive; sign arithmetic with its three differences a score made a
+// block with the mask take 2.3 us longer than one without.
+template <int T>
+__device__ __forceinline__ void hide(f32x16 (&s)[T], int hi, int lo, int sink) {
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    const uint32_t seen = low_bits(hi + 1 - 32 * t) & (~low_bits(lo - 32 * t) | low_bits(sink - 32 * t));
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const uint32_t keep = (uint32_t)__builtin_amdgcn_sbfe((int)seen, 8 * (r >> 2) + (r & 3), 1);
+      s[t][r] = __uint_as_float((__float_as_uint(s[t][r]) & keep) | (0xff800000u & ~keep));
+    }
+  }
 }
 
 // One step of the online softmax over N scores of the lane's row (the other
@@ -307,13 +338,16 @@ struct Stream {
   __device__ __forceinline__ bool missing(int key, int id) const {
     return PAGED && key < keys && (uint32_t)id >= (uint32_t)pages;
   }
+  // Without a branch: a range of 0 fetches nothing, whatever the base.
   __device__ __forceinline__ i32x4 rsrc(const char* base, uint32_t page_bytes, int pitch, int key, int id) const {
     const int n = valid(key, id);
     if constexpr (PAGED)
       base += (uint64_t)(uint32_t)id * page_bytes + (uint64_t)(uint32_t)(key & ((1 << shift) - 1)) * (uint32_t)pitch;
     else
       base += (int64_t)key * pitch;
-    return buffer_rsrc(n ? base : nullptr, n ? (n - 1) * pitch + ROW_BYTES : 0);
+    const int range = (n - 1) * pitch + ROW_BYTES;
+    const i32x4 rs = buffer_rsrc(base, n > 0 ? range : 0);
+    return i32x4{uniform(rs[0]), uniform(rs[1]), uniform(rs[2]), rs[3]};
   }
   __device__ __forceinline__ i32x4 k_rsrc(int key, int id) const { return rsrc(k, ks_b, ks_n, key, id); }
   __device__ __forceinline__ i32x4 v_rsrc(int key, int id) const { return rsrc(v, vs_b, vs_n, key, id); }
@@ -373,7 +407,8 @@ __device__ __forceinline__ bool is_nan(float x) { return !(x == x); }
 // The row kernel: requests of few rows (decode, a few tokens behind a cache).
 // Every key is read once and that read is the bound, so the kernel is laid out
 // for bytes in flight and even shares. A workgroup is 4 waves, two of them to a CU
-// (64 KiB of LDS each); a wave takes 32 of a block's 128 keys for itself, its own
+// (64 KiB of LDS each), or beside the tile kernel's 8 waves, every other block
+// for each half; a wave takes 32 of a block's 128 keys for itself, its own
 // LDS slots (8 KiB of K, 8 KiB of V), statistics and O, so the key loop has no
 // barrier: K(j + 1) is loaded once K(j) is in registers, V(j + 1) after the
 // products of block j. The four results are joined in LDS at an item's end.
@@ -385,17 +420,11 @@ __device__ __forceinline__ bool is_nan(float x) { return !(x == x); }
 // workgroup has at most two, its first and its last), and the merge kernel joins
 // an item's pieces.
 constexpr int RT = 32;
-constexpr int RW = 4;                       // waves
-constexpr int RTHREADS = RW * 64;
 constexpr int RSLOT = 32 * ROW_BYTES;       // 32 keys of K or V
-constexpr int kRowsLds = RW * 2 * RSLOT;
-constexpr int kRowsGroups = 512;            // two a CU
+constexpr int rows_lds(int waves) { return waves * 2 * RSLOT; }
+constexpr int kRowsGroups = 512;            // of 4 waves, two a CU; half as many of 8 waves
 constexpr int kMinShare = 2;                // blocks a share holds at least
 constexpr int DESC_INTS = 8;                // ints of a descriptor
-
-struct Piece {
-  int b, hk, tile, first, last;             // item, and the workgroups that share it
-};
 
 template <bool PAGED>
 __device__ __forceinline__ int row_tiles(const AttnArgs& a, const Request& r) {
@@ -412,7 +441,7 @@ __device__ __forceinline__ Blocks uniform(const Blocks& k) {
   return Blocks{uniform(k.ns), uniform(k.w0), uniform(k.w1), uniform(k.f0), uniform(k.f1)};
 }
 
-template <bool BF, bool PAGED>
+template <bool BF, bool PAGED, int RW>
 __device__ __forceinline__ void row_item(const AttnArgs& a, const Request& r, int b, int hk, int tile, int s0, int s1,
                                          int nblk, int slot, char* lds, float* st_m, float* st_l) {
   // Opaque, so that nothing derived from it is kept across the items.
@@ -448,14 +477,14 @@ __device__ __forceinline__ void row_item(const AttnArgs& a, const Request& r, in
   const uint32_t vdst = kdst + RSLOT;
   bool bad = r.bad;
   // Keys of this wave in block s of the list (past the piece: no keys).
-  auto key_of = [&](int s) { return s < s1 ? block_at(s) * BLOCK + wave * 32 : 1 << 30; };
+  auto key_of = [&](int s) { return s < s1 ? block_at(s) * BLOCK + (wave & 3) * 32 : 1 << 30; };
   auto load_k = [&](int key, const int (&id)[2]) {
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       bad |= st.missing(key + 16 * g, id[g]);
       const i32x4 rs = st.k_rsrc(key + 16 * g, id[g]);
 #pragma unroll
-      for (int x = 0; x < 4; ++x) dma_to_lds(rs, kdst + (4 * g + x) * 1024, koff[x], 4 * x * st.ks_n);
+      for (int x = 0; x < 4; ++x) dma_to_lds_late(rs, kdst + (4 * g + x) * 1024, koff[x], 4 * x * st.ks_n);
     }
   };
   auto load_v = [&](int key, const int (&id)[2]) {
@@ -463,7 +492,7 @@ __device__ __forceinline__ void row_item(const AttnArgs& a, const Request& r, in
     for (int g = 0; g < 2; ++g) {
       const i32x4 rs = st.v_rsrc(key + 16 * g, id[g]);
 #pragma unroll
-      for (int x = 0; x < 4; ++x) dma_to_lds(rs, vdst + (4 * g + x) * 1024, voff, 4 * x * st.vs_n);
+      for (int x = 0; x < 4; ++x) dma_to_lds_late(rs, vdst + (4 * g + x) * 1024, voff, 4 * x * st.vs_n);
     }
   };
   auto pages_of = [&](int key, int (&id)[2]) {
@@ -473,14 +502,15 @@ __device__ __forceinline__ void row_item(const AttnArgs& a, const Request& r, in
 
   const char* qrow = a.q + b * a.qs_b + (int64_t)(r.row0 + i) * a.qs_n + head * a.qs_h;
   int id[2], next[2];
-  int key = key_of(s0);
+  int key = key_of(s0 + (wave >> 2));
   pages_of(key, id);
   h8 qf[8];
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk) qf[kk] = *reinterpret_cast<const h8*>(qrow + (kk * 2 + hf) * 16);
   load_k(key, id);
   load_v(key, id);
-  int key_next = key_of(s0 + 1);
+  constexpr int STEP = RW / 4;              // blocks a round of the waves covers
+  int key_next = key_of(s0 + (wave >> 2) + STEP);
   pages_of(key_next, next);
   // The compiler waits for its own loads here, before the key loop.
 #pragma unroll
@@ -497,7 +527,7 @@ __device__ __forceinline__ void row_item(const AttnArgs& a, const Request& r, in
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt) acc[dt] = f32x16{};
   float m = -INFINITY, l = 0.f;
-  for (int s = s0; s < s1; ++s) {
+  for (int s = s0 + (wave >> 2); s < s1; s += STEP) {
     wait_loads<8>();                        // K has landed; V may be in flight
     f32x16 sc[1];
     sc[0] = f32x16{};
@@ -509,8 +539,7 @@ __device__ __forceinline__ void row_item(const AttnArgs& a, const Request& r, in
     if (!whole(key)) {
       const int base = key + 4 * hf;
       const int hi = min(pos, r.keys - 1) - base, lo = pos - a.window + 1 - base, sink = a.sinks - base;
-#pragma unroll
-      for (int x = 0; x < 16; ++x) sc[0][x] = masked(sc[0][x], 8 * (x >> 2) + (x & 3), hi, lo, sink);
+      hide(sc, hi, lo, sink);
     }
     h8 p[2];
     softmax_step<BF, 1>(sc, p, m, l, acc, a.c, [](int) {});
@@ -526,7 +555,7 @@ __device__ __forceinline__ void row_item(const AttnArgs& a, const Request& r, in
     wait_lds();
     load_v(key_next, next);
     key = key_next;
-    key_next = key_of(s + 2);
+    key_next = key_of(s + 2 * STEP);
     pages_of(key_next, next);
   }
 
@@ -546,7 +575,11 @@ __device__ __forceinline__ void row_item(const AttnArgs& a, const Request& r, in
       *reinterpret_cast<float4*>(kslot + l32 * 512 + (((dt * 8 + 2 * g + hf) ^ l32) << 4)) = val;
     }
   __syncthreads();
-  // 8 threads a row, 16 dims each: 8 at 8t and 8 at 64 + 8t.
+  // The first 4 waves: 8 threads a row, 16 dims each, 8 at 8t and 8 at 64 + 8t.
+  if (RW > 4 && wave >= 4) {
+    __syncthreads();
+    return;
+  }
   const int n = tid >> 3, t = tid & 7;
   const int orow = tile * RT + n;
   float M = -INFINITY;
@@ -628,14 +661,13 @@ __device__ __forceinline__ void row_item(const AttnArgs& a, const Request& r, in
   }
 }
 
-template <bool BF, bool PAGED>
-__global__ void __launch_bounds__(RTHREADS) __attribute__((amdgpu_waves_per_eu(2, 2)))
-fa_serve_rows_kernel(AttnArgs a) {
-  extern __shared__ __attribute__((aligned(16))) char lds[];
+// The share of workgroup g, of RW waves.
+template <bool BF, bool PAGED, int RW>
+__device__ __forceinline__ void rows_share(const AttnArgs& a, int g, char* lds) {
+  constexpr int RTHREADS = RW * 64;
   __shared__ float st_m[RW * RT], st_l[RW * RT];
   __shared__ uint32_t wave_sum[RW];
   __shared__ int found[2];
-  __shared__ uint32_t found_at;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   // Blocks of all items before this thread's run of requests, and of all.
   const int per = (a.batch + RTHREADS - 1) / RTHREADS;
@@ -646,12 +678,7 @@ fa_serve_rows_kernel(AttnArgs a) {
   };
   uint32_t mine = 0;
   for (int b = b0; b < b1; ++b) mine += cost(request<PAGED>(a, b));
-  uint32_t sum = mine;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t other = __shfl_up(sum, d);
-    if (lane >= d) sum += other;
-  }
+  const uint32_t sum = lanes_sum(mine);
   if (lane == 63) wave_sum[wave] = sum;
   __syncthreads();
   uint32_t before = sum - mine, total = 0;
@@ -660,7 +687,6 @@ fa_serve_rows_kernel(AttnArgs a) {
     if (w < wave) before += wave_sum[w];
     total += wave_sum[w];
   }
-  const int g = blockIdx.x;
   total = uniform(total);
   const uint32_t share = max(uniform((total + a.groups - 1) / a.groups), (uint32_t)kMinShare);
   uint32_t x = share * g;
@@ -679,11 +705,11 @@ fa_serve_rows_kernel(AttnArgs a) {
       at += n;
     }
     found[0] = b;
-    found_at = at;
+    found[1] = (int)at;
   }
   __syncthreads();
   int b = __builtin_amdgcn_readfirstlane(found[0]);
-  uint32_t at = uniform(found_at);          // where request b's blocks start
+  uint32_t at = uniform((uint32_t)found[1]);          // where request b's blocks start
   bool head = true;
   for (; b < a.batch; ++b) {
     const Request r = uniform_request<PAGED>(a, b);
@@ -706,13 +732,20 @@ fa_serve_rows_kernel(AttnArgs a) {
           desc[4] = (int)((start + nblk - 1) / share);
         }
         head = false;
-        row_item<BF, PAGED>(a, r, b, hk, tile, s0, s1, nblk, 2 * g + (s0 == 0), lds, st_m, st_l);
+        row_item<BF, PAGED, RW>(a, r, b, hk, tile, s0, s1, nblk, 2 * g + (s0 == 0), lds, st_m, st_l);
         x += s1 - s0;
       }
       at = stop;
     }
     if (x >= end) break;
   }
+}
+
+template <bool BF, bool PAGED>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+fa_serve_rows_kernel(AttnArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  rows_share<BF, PAGED, 4>(a, blockIdx.x, lds);
 }
 
 // Joins the pieces of the items that several workgroups share:
@@ -727,16 +760,16 @@ fa_serve_rows_kernel(AttnArgs a) {
 // 16.6 us for 8 rows of 2 or 3 (64 requests).
 constexpr int kFewPieces = 32;
 template <bool BF, bool PAGED>
-__global__ void __launch_bounds__(256) fa_serve_rows_merge_kernel(AttnArgs a) {
+__device__ __forceinline__ void merge_rows(const AttnArgs& a, int block) {
   __shared__ float weight[kRowsGroups];
   __shared__ float red[32][36];             // padded: 8 rows of 4 lanes' dims at a time
   __shared__ float wave_red[4];
-  const int* desc = a.desc + (blockIdx.x + 1) * DESC_INTS;
+  const int* desc = a.desc + (block + 1) * DESC_INTS;
   const int first = desc[3];
   if (first < 0) return;
   const int b = desc[0], hk = desc[1], tile = desc[2], last = desc[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int boundaries = last - first, pieces = boundaries + 1, mine = (int)blockIdx.x - first;
+  const int boundaries = last - first, pieces = boundaries + 1, mine = block - first;
   const Request r = request<PAGED>(a, b);
   const int rows = min(r.n * a.group - tile * RT, RT);
   auto piece = [&](int s) { return (int64_t)(2 * (first + s) + (s == 0)); };
@@ -878,7 +911,7 @@ __device__ __forceinline__ int tile_count(const AttnArgs& a, const Request& r) {
   return rows > a.rows_max ? (int)((rows + TT - 1) / TT) : 0;
 }
 // At least the blocks of any tile of the request.
-__device__ __forceinline__ int tile_blocks(const AttnArgs& a, const Request& r) {
+__host__ __device__ __forceinline__ int tile_blocks(const AttnArgs& a, const Request& r) {
   const Blocks all = blocks(a, r, r.pos, r.pos + r.n - 1);
   const int span = min(TT / a.group + 2, r.n);
   const int64_t near = ((int64_t)a.window + span + BLOCK - 1) / BLOCK + 1 + (a.sinks + BLOCK - 1) / BLOCK;
@@ -889,6 +922,7 @@ __device__ __forceinline__ int tile_blocks(const AttnArgs& a, const Request& r) 
 struct Item {
   int b, hk, tile, part, parts, length;     // length: blocks of a part
   int index, tile_index;                    // place among all parts, all tiles
+  Request r;
 };
 
 template <bool BF, bool PAGED>
@@ -898,7 +932,7 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
   const int lane = tid & 63, l32 = lane & 31, hf = lane >> 5, lr = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int grp = wave >> 2, dw = wave & 3;
-  const Request r = uniform_request<PAGED>(a, it.b);
+  const Request& r = it.r;
   const int b = it.b, hk = it.hk;
   const int rows = r.n * a.group;
   const int row0 = it.tile * TT + wave * 32;
@@ -949,34 +983,44 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk) qf[kk] = *reinterpret_cast<const h8*>(qrow + (kk * 2 + hf) * 16);
 
-  // Loads: instruction x of group 1's wave dw fills rows 16x + 4dw .. + 3 of a block, one
-  // of the 16-key groups.
-  const int koff = (4 * dw + lr) * st.ks_n + ((lane & 15) ^ (4 * dw + lr)) * 16;
-  const int voff = (4 * dw + lr) * st.vs_n + ((lane & 15) ^ (4 * lr)) * 16;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+  // Loads: group 1's wave dw fills rows 32 dw .. + 31 of a block, two 16-key groups
+  // and so two descriptors for its 8 instructions of 4 rows each.
+  int koff[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) koff[x] = lr * st.ks_n + ((lane & 15) ^ (4 * x + lr)) * 16;
+  const int voff = lr * st.vs_n + ((lane & 15) ^ (4 * lr)) * 16;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds + dw * (32 * ROW_BYTES);
   bool bad = r.bad;
-  // Pages of the next K block to load, of the V block to load beside it and of the
-  // K block after: lane x holds that of the block's 16-key group x % 8.
-  int kid = 0, vid = 0, nid = 0;
-  int kkey = 0, vkey = 0, nkey = 0;         // first keys of those blocks
+  // First keys (of this wave) and pages of the next K block to load, of the V block to
+  // load beside it and of the K block after.
+  int kid[2], vid[2], nid[2], kkey = 0, vkey = 0, nkey = 0;
   auto fetch = [&](int s) {
-    nkey = s < nblk ? block_at(s) * BLOCK : 1 << 30;
-    nid = st.page(nkey + 16 * (lane & 7));
+    nkey = s < nblk ? block_at(s) * BLOCK + 32 * dw : 1 << 30;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) nid[g] = uniform(st.page(nkey + 16 * g));
   };
   auto shift_ids = [&]() {
     vkey = kkey;
     kkey = nkey;
-    vid = kid;
-    kid = nid;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      vid[g] = kid[g];
+      kid[g] = nid[g];
+    }
   };
+  i32x4 rs;                                 // of the group that is being loaded
   auto load_k = [&](int x, int slot) {
-    const int id = __builtin_amdgcn_readlane(kid, x);
-    bad |= st.missing(kkey + 16 * x, id);
-    dma_to_lds(st.k_rsrc(kkey + 16 * x, id), lds0 + slot * TBLOCK + (4 * x + dw) * 1024, koff, 0);
+    const int g = x >> 2;
+    if ((x & 3) == 0) {
+      bad |= st.missing(kkey + 16 * g, kid[g]);
+      rs = st.k_rsrc(kkey + 16 * g, kid[g]);
+    }
+    dma_to_lds_late(rs, lds0 + slot * TBLOCK + x * 1024, koff[x & 3], 4 * (x & 3) * st.ks_n);
   };
   auto load_v = [&](int x, int slot) {
-    const int id = __builtin_amdgcn_readlane(vid, x);
-    dma_to_lds(st.v_rsrc(vkey + 16 * x, id), lds0 + (2 + slot) * TBLOCK + (4 * x + dw) * 1024, voff, 0);
+    const int g = x >> 2;
+    if ((x & 3) == 0) rs = st.v_rsrc(vkey + 16 * g, vid[g]);
+    dma_to_lds_late(rs, lds0 + (2 + slot) * TBLOCK + x * 1024, voff, 4 * (x & 3) * st.vs_n);
   };
 
   f32x16 acc[4], s[4];
@@ -1030,10 +1074,7 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
     if constexpr (decltype(with_mask)::value) {
       const int base = block_at(j) * BLOCK + 4 * hf;
       const int hi = min(pos, r.keys - 1) - base, lo = pos - window + 1 - base, sink = sinks - base;
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int x = 0; x < 16; ++x) s[t][x] = masked(s[t][x], 32 * t + 8 * (x >> 2) + (x & 3), hi, lo, sink);
+      hide(s, hi, lo, sink);
     }
     softmax_step<BF, 4>(s, p, m, l, acc, c, at);
   };
@@ -1218,6 +1259,20 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
   }
 }
 
+// Cost of a launch whose tiles, the longest of `longest` blocks, are cut into
+// parts of `length` blocks, `items` of them (p = 1: uncut, all of them in the one round
+// that fewer tiles than CUs take).
+__host__ __device__ inline float cut_cost(int p, int longest, int length, int64_t items) {
+  if (p == 1) return longest + kWholeCost;
+  if (items > kTileItems) return 1e30f;
+  const float rounds = (float)((items + kTileGroups - 1) / kTileGroups);
+  return rounds * (length + kPartCost) + kMergeCost + kMergeShare * items;
+}
+__host__ __device__ inline int cut_length(int p, int longest) {
+  const int n = (longest + p - 1) / p;
+  return n > 1 ? n : 1;
+}
+
 // Which item a workgroup has. The 8 dies take workgroups in turn (die = workgroup
 // % 8), and the tiles that read the same keys should be on one die at a time, so
 // that its L2 fetches them once, while every die gets its share of long and short
@@ -1225,165 +1280,233 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
 // and, of request b's tiles counted from the last (the longest come first), those
 // with number (x / h + b) mod (8 / h). Parts: the tiles of a part are consecutive,
 // and each die has an eighth of all parts, consecutive ones.
+struct Dies {
+  int die, h, step, heads_kv;
+  __device__ __forceinline__ Dies(int die, int heads_kv)
+      : die(die), h(min(heads_kv & -heads_kv, 8)), step(8 / h), heads_kv(heads_kv) {}
+  __device__ __forceinline__ int first(int b) const { return (die / h + b) & (step - 1); }
+  // Whole tiles of request b that the die takes of one head, and of all its heads.
+  __device__ __forceinline__ int tiles_of(int b, int tiles) const {
+    return max(0, (tiles - first(b) + step - 1) / step);
+  }
+  __device__ __forceinline__ int items_of(int b, int tiles) const { return heads_kv / h * tiles_of(b, tiles); }
+  // The rel-th of these.
+  __device__ __forceinline__ void whole(int b, int tiles, int rel, Item& it) const {
+    const int here = tiles_of(b, tiles), unit = rel / here;
+    it.b = b;
+    it.hk = unit * h + die % h;
+    it.tile = tiles - 1 - (first(b) + (rel - unit * here) * step);
+    it.part = it.index = it.tile_index = 0;
+    it.parts = 1;
+  }
+  // The rel-th part of request b, whose parts and tiles others precede.
+  __device__ __forceinline__ void part(int b, int tiles, int parts, int rel, int before, int tiles_before, Item& it) const {
+    const int unit = rel / tiles;
+    it.b = b;
+    it.hk = unit / parts;
+    it.part = unit - it.hk * parts;
+    it.tile = tiles - 1 - (rel - unit * tiles);
+    it.parts = parts;
+    it.tile_index = tiles_before + it.hk * tiles + it.tile;
+    it.index = before + (it.hk * tiles + it.tile) * parts + it.part;
+  }
+  // This die's part number `slot` of `total`; total if it has no such part.
+  __device__ __forceinline__ uint32_t eighth(uint32_t slot, uint32_t total) const {
+    const uint32_t n = (total + 7) / 8;
+    return slot < n ? die * n + slot : total;
+  }
+};
+
+// The item of workgroup `slot` of its die, if it has one. Contiguous: every request
+// is alike, and the host has chosen the cut.
 template <bool BF, bool PAGED>
+__device__ __forceinline__ bool find_item(const AttnArgs& a, const Dies& d, uint32_t slot, char* lds, Item& it) {
+  const int tid = threadIdx.x;
+  if constexpr (!PAGED) {
+    const Request r = request<PAGED>(a, 0);
+    const int tiles = tile_count<PAGED>(a, r);
+    it.r = r;
+    it.length = a.length;
+    if (a.length < kUncut) {
+      const int parts = (tile_blocks(a, r) + a.length - 1) / a.length, each = a.heads_kv * tiles * parts;
+      const uint32_t total = (uint32_t)a.batch * each, x = d.eighth(slot, total);
+      if (x >= total) return false;
+      const int b = x / each;
+      d.part(b, tiles, parts, (int)(x - b * each), b * each, b * a.heads_kv * tiles, it);
+    } else {
+      // `step` consecutive requests' tiles of a head are dealt to the dies evenly.
+      const uint32_t each = (uint32_t)(a.heads_kv / d.h * tiles);
+      int b = (int)(slot / each) * d.step, rel = (int)(slot % each);
+      while (b < a.batch && rel >= d.items_of(b, tiles)) rel -= d.items_of(b++, tiles);
+      if (b >= a.batch) return false;
+      d.whole(b, tiles, rel, it);
+    }
+  } else {
+    __shared__ uint32_t wave_sum[TTHREADS / 64][3];
+    __shared__ float costs[kCuts];
+    __shared__ int longest;
+    __shared__ Item found;
+    const int lane = tid & 63, wave = tid >> 6;
+    const int per = (a.batch + TTHREADS - 1) / TTHREADS;
+    const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
+    if (tid == 0) {
+      longest = 0;
+      found.b = -1;
+      found.length = kUncut;
+    }
+    __syncthreads();
+    // All tiles (at most 256 a request: only fewer in all matter) and this die's
+    // whole ones before this thread's run of requests.
+    uint32_t tiles_mine = 0, whole_mine = 0;
+    int2* const loads = reinterpret_cast<int2*>(lds);   // of every request: tiles, blocks
+    for (int b = b0; b < b1; ++b) {
+      const Request r = request<PAGED>(a, b);
+      const int tiles = tile_count<PAGED>(a, r), n = tiles ? tile_blocks(a, r) : 0;
+      tiles_mine += min((int64_t)a.heads_kv * tiles, (int64_t)kTileGroups);
+      whole_mine += tiles ? d.items_of(b, tiles) : 0;
+      if (a.split) {
+        loads[b] = int2{(int)min((int64_t)a.heads_kv * tiles, (int64_t)kTileGroups), n};
+        if (n) atomicMax(&longest, n);
+      }
+    }
+    const uint32_t scan_t = lanes_sum(tiles_mine), scan_w = lanes_sum(whole_mine);
+    if (lane == 63) {
+      wave_sum[wave][0] = scan_t;
+      wave_sum[wave][1] = scan_w;
+    }
+    __syncthreads();
+    uint32_t all_tiles = 0, tiles_before = scan_t - tiles_mine, before = scan_w - whole_mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < TTHREADS / 64; ++w) {
+      if (w < wave) {
+        tiles_before += wave_sum[w][0];
+        before += wave_sum[w][1];
+      }
+      all_tiles += wave_sum[w][0];
+      total += wave_sum[w][1];
+    }
+    // Fewer tiles than CUs: cut them if that is modelled to be faster. Wave w looks
+    // at cuts of the longest tile into w + 1, w + 9, .. parts.
+    int length = kUncut;
+    const bool few = a.split && all_tiles < kTileGroups;     // uniform
+    if (few) {
+      for (int p = wave + 1; p <= kCuts; p += TTHREADS / 64) {
+        const int n = cut_length(p, longest);
+        int items = 0;
+        for (int b = lane; b < a.batch; b += 64) items += loads[b].x * ((loads[b].y + n - 1) / n);
+        items = (int)lanes_sum((uint32_t)items);
+        if (lane == 63) costs[p - 1] = cut_cost(p, longest, n, items);
+      }
+      __syncthreads();
+      int best = 1;
+      for (int p = 2; p <= kCuts; ++p)
+        if (costs[p - 1] < costs[best - 1]) best = p;
+      if (best > 1) length = cut_length(best, longest);
+    }
+    const bool cut = length < kUncut;
+    if (a.split && blockIdx.x == 0 && tid == 0) a.tdesc[0] = cut ? (int)all_tiles : 0;
+    uint32_t mine = whole_mine, x = slot;
+    if (cut) {
+      mine = 0;
+      for (int b = b0; b < b1; ++b) mine += loads[b].x * ((loads[b].y + length - 1) / length);
+      const uint32_t scan = lanes_sum(mine);
+      if (lane == 63) wave_sum[wave][2] = scan;
+      __syncthreads();
+      before = scan - mine;
+      total = 0;
+#pragma unroll
+      for (int w = 0; w < TTHREADS / 64; ++w) {
+        if (w < wave) before += wave_sum[w][2];
+        total += wave_sum[w][2];
+      }
+      x = d.eighth(slot, total);
+    }
+    if (x >= total) return false;           // uniform
+    if (before <= x && x - before < mine) {
+      uint32_t rel = x - before;
+      for (int b = b0; b < b1; ++b) {
+        const Request r = request<PAGED>(a, b);
+        const int tiles = tile_count<PAGED>(a, r);
+        if (!tiles) continue;
+        const int parts = cut ? (loads[b].y + length - 1) / length : 1;
+        const uint32_t n = cut ? (uint32_t)(a.heads_kv * tiles * parts) : (uint32_t)d.items_of(b, tiles);
+        if (rel >= n) {
+          rel -= n;
+          before += n;
+          tiles_before += a.heads_kv * tiles;
+          continue;
+        }
+        Item mine;
+        if (cut)
+          d.part(b, tiles, parts, (int)rel, (int)before, (int)tiles_before, mine);
+        else
+          d.whole(b, tiles, (int)rel, mine);
+        mine.length = length;
+        mine.r = r;
+        found = mine;
+        break;
+      }
+    }
+    __syncthreads();
+    it = found;
+    if (it.b < 0) return false;             // requests that overlap, counted past 32 bits
+  }
+  it.b = uniform(it.b);
+  it.hk = uniform(it.hk);
+  it.tile = uniform(it.tile);
+  it.part = uniform(it.part);
+  it.parts = uniform(it.parts);
+  it.length = uniform(it.length);
+  it.index = uniform(it.index);
+  it.tile_index = uniform(it.tile_index);
+  it.r.row0 = uniform(it.r.row0);
+  it.r.n = uniform(it.r.n);
+  it.r.pos = uniform(it.r.pos);
+  it.r.keys = uniform(it.r.keys);
+  it.r.bad = uniform((int)it.r.bad);
+  return true;
+}
+
+// In a mixed launch the workgroups from a.tile_groups on do the row kernel's work, in
+// 8 waves: they fill the CUs that have no long tile (22 decoding requests beside two
+// chunks of 1000 tokens: 193 us, one kernel after the other 214).
+template <bool BF, bool PAGED, bool MIXED>
 __global__ void __launch_bounds__(TTHREADS) __attribute__((amdgpu_waves_per_eu(2, 2)))
 fa_serve_tiles_kernel(AttnArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  __shared__ uint64_t wave_sum[TTHREADS / 64][5];
-  __shared__ float cut_cost[kCuts];
-  __shared__ int found[8];
   __shared__ int flag;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int die = blockIdx.x & 7, slot0 = blockIdx.x >> 3;
-  const int h = min(a.heads_kv & -a.heads_kv, 8), step = 8 / h;
-  const int per = (a.batch + TTHREADS - 1) / TTHREADS;
-  const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
-  auto wave_scan = [&](uint64_t v) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint64_t other = __shfl_up(v, d);
-      if (lane >= d) v += other;
+  if constexpr (MIXED)
+    if ((int)blockIdx.x >= a.tile_groups) {
+      rows_share<BF, PAGED, 8>(a, blockIdx.x - a.tile_groups, lds);
+      return;
     }
-    return v;
-  };
-  // Tiles and blocks of all requests and the longest tile's.
-  uint64_t tiles_mine = 0, blocks_mine = 0;
-  int longest = 0;
-  int2* const loads = reinterpret_cast<int2*>(lds);   // of every request: tiles, blocks
-  for (int b = b0; b < b1; ++b) {
-    const Request r = request<PAGED>(a, b);
-    const int t = a.heads_kv * tile_count<PAGED>(a, r), n = t ? tile_blocks(a, r) : 0;
-    if (a.split) loads[b] = int2{t, n};
-    tiles_mine += t;
-    blocks_mine += (uint64_t)t * n;
-    longest = max(longest, n);
-  }
-  const uint64_t scan_b = wave_scan(blocks_mine), scan_t = wave_scan(tiles_mine);
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) longest = max(longest, __shfl_xor(longest, d));
-  if (lane == 63) {
-    wave_sum[wave][0] = scan_b;
-    wave_sum[wave][1] = scan_t;
-    wave_sum[wave][2] = longest;
-  }
-  __syncthreads();
-  uint64_t total_b = 0, total_t = 0, tiles_before = scan_t - tiles_mine;
-#pragma unroll
-  for (int w = 0; w < TTHREADS / 64; ++w) {
-    if (w < wave) tiles_before += wave_sum[w][1];
-    total_b += wave_sum[w][0];
-    total_t += wave_sum[w][1];
-    longest = max(longest, (int)wave_sum[w][2]);
-  }
-  // Cut if there are fewer tiles than CUs and that is modelled to be faster: with
-  // parts of at most `length` blocks, a round of parts for every 256 of them. Wave w
-  // looks at cuts of the longest tile into w + 1, w + 9, .. parts.
-  int length = 1 << 30;
-  if (a.split && total_t < kTileGroups) {   // uniform
-    for (int p = wave + 1; p <= kCuts; p += TTHREADS / 64) {
-      const int n = max((longest + p - 1) / p, 1);
-      int items = 0;
-      for (int b = lane; b < a.batch; b += 64) items += loads[b].x * ((loads[b].y + n - 1) / n);
-#pragma unroll
-      for (int d = 32; d >= 1; d >>= 1) items += __shfl_xor(items, d);
-      const float rounds = (float)((items + kTileGroups - 1) / kTileGroups);
-      // Uncut tiles of different lengths share the one round there is.
-      const float cost = p == 1 ? longest + kWholeCost
-                                : rounds * (n + kPartCost) + kMergeCost + kMergeShare * items;
-      if (lane == 0) cut_cost[p - 1] = items <= kTileItems ? cost : INFINITY;
-    }
-    __syncthreads();
-    int best = 1;
-    for (int p = 2; p <= kCuts; ++p)
-      if (cut_cost[p - 1] < cut_cost[best - 1]) best = p;
-    if (best > 1) length = uniform(max((longest + best - 1) / best, 1));
-  }
-  const bool split = length < 1 << 30;
-  if (a.split && blockIdx.x == 0 && tid == 0) a.tdesc[0] = split ? (int)total_t : 0;
-  auto parts_of = [&](const Request& r) { return split ? (tile_blocks(a, r) + length - 1) / length : 1; };
-  // Of whole tiles, those of request b that die `die` takes.
-  auto first_of = [&](int b) { return (die / h + b) % step; };
-  auto tiles_of = [&](int b, int tiles) { return max(0, (tiles - first_of(b) + step - 1) / step); };
-  auto items_of = [&](int b, int tiles, int parts) {
-    return split ? a.heads_kv * tiles * parts : a.heads_kv / h * tiles_of(b, tiles);
-  };
-  uint64_t mine = 0;
-  for (int b = b0; b < b1; ++b) {
-    const Request r = request<PAGED>(a, b);
-    const int tiles = tile_count<PAGED>(a, r);
-    if (tiles) mine += items_of(b, tiles, parts_of(r));
-  }
-  const uint64_t scan_m = wave_scan(mine);
-  if (lane == 63) wave_sum[wave][3] = scan_m;
-  __syncthreads();
-  uint64_t before = scan_m - mine, total = 0;
-#pragma unroll
-  for (int w = 0; w < TTHREADS / 64; ++w) {
-    if (w < wave) before += wave_sum[w][3];
-    total += wave_sum[w][3];
-  }
-  uint64_t x = slot0;
-  if (split) {
-    const uint64_t eighth = (total + 7) / 8;
-    x = slot0 < eighth ? die * eighth + slot0 : total;
-  }
-  if (x >= total) return;                   // uniform
-  if (before <= x && x < before + mine) {
-    uint64_t at = before, t_at = tiles_before;
-    for (int b = b0;; ++b) {
-      const Request r = request<PAGED>(a, b);
-      const int tiles = tile_count<PAGED>(a, r);
-      if (!tiles) continue;
-      const int parts = parts_of(r), n = items_of(b, tiles, parts);
-      if (x >= at + n) {
-        at += n;
-        t_at += (uint64_t)a.heads_kv * tiles;
-        continue;
-      }
-      const int rel = (int)(x - at), here = split ? tiles : tiles_of(b, tiles), unit = rel / here;
-      const int hk = split ? unit / parts : unit * h + die % h;
-      const int tile = tiles - 1 - (split ? rel % here : first_of(b) + rel % here * step);
-      const int part = split ? unit % parts : 0;
-      found[0] = b;
-      found[1] = hk;
-      found[2] = tile;
-      found[3] = part;
-      found[4] = parts;
-      found[5] = (int)at + (hk * tiles + tile) * parts + part;
-      found[6] = (int)t_at + hk * tiles + tile;
-      break;
-    }
-  }
-  __syncthreads();
+  const Dies d(blockIdx.x & 7, a.heads_kv);
   Item it;
-  it.b = uniform(found[0]);
-  it.hk = uniform(found[1]);
-  it.tile = uniform(found[2]);
-  it.part = uniform(found[3]);
-  it.parts = uniform(found[4]);
-  it.index = uniform(found[5]);
-  it.tile_index = uniform(found[6]);
-  it.length = length;
-  if (split && it.part == 0 && tid == 0) {
-    int* d = a.tdesc + (it.tile_index + 1) * DESC_INTS;
-    d[0] = it.b;
-    d[1] = it.hk;
-    d[2] = it.tile;
-    d[3] = it.index;
-    d[4] = it.parts;
+  const bool some = find_item<BF, PAGED>(a, d, blockIdx.x >> 3, lds, it);
+  if (!PAGED && blockIdx.x == 0 && threadIdx.x == 0 && a.split)
+    a.tdesc[0] = a.length < kUncut ? a.batch * a.heads_kv * tile_count<PAGED>(a, request<PAGED>(a, 0)) : 0;
+  if (!some) return;
+  if (it.length < kUncut && it.part == 0 && threadIdx.x == 0) {
+    int* desc = a.tdesc + (it.tile_index + 1) * DESC_INTS;
+    desc[0] = it.b;
+    desc[1] = it.hk;
+    desc[2] = it.tile;
+    desc[3] = it.index;
+    desc[4] = it.parts;
   }
+  __syncthreads();                          // the LDS that find_item used is free
   tile_item<BF, PAGED>(a, it, lds, &flag);
 }
 
 // Joins the parts of the tiles, 8 rows a workgroup, 32 lanes a row (4 dims each).
 template <bool BF, bool PAGED>
-__global__ void __launch_bounds__(256) fa_serve_tiles_merge_kernel(AttnArgs a) {
-  const int t = blockIdx.x >> 5;
+__device__ __forceinline__ void merge_tiles(const AttnArgs& a, int block) {
+  const int t = block >> 5;
   if (t >= a.tdesc[0]) return;
   const int* d = a.tdesc + (t + 1) * DESC_INTS;
   const int parts = d[4];
   if (parts < 2) return;
-  const int b = d[0], hk = d[1], n = (blockIdx.x & 31) * 8 + (threadIdx.x >> 5), dim = (threadIdx.x & 31) * 4;
+  const int b = d[0], hk = d[1], n = (block & 31) * 8 + (threadIdx.x >> 5), dim = (threadIdx.x & 31) * 4;
   const Request r = request<PAGED>(a, b);
   const int row = d[2] * TT + n;
   if (row >= r.n * a.group) return;
@@ -1412,6 +1535,25 @@ __global__ void __launch_bounds__(256) fa_serve_tiles_merge_kernel(AttnArgs a) {
     a.lse[b * a.ls_b + (int64_t)(r.row0 + i) * a.ls_n + head * a.ls_h] = M == -INFINITY ? M : M + logf(total);
 }
 
+// The joins of a launch: of the row kernel's pieces (a.groups - 1 workgroups), of the
+// tiles' parts, or both.
+template <bool BF, bool PAGED>
+__global__ void __launch_bounds__(256) fa_serve_rows_merge_kernel(AttnArgs a) {
+  merge_rows<BF, PAGED>(a, blockIdx.x);
+}
+template <bool BF, bool PAGED>
+__global__ void __launch_bounds__(256) fa_serve_tiles_merge_kernel(AttnArgs a) {
+  merge_tiles<BF, PAGED>(a, blockIdx.x);
+}
+template <bool BF>
+__global__ void __launch_bounds__(256) fa_serve_mixed_merge_kernel(AttnArgs a) {
+  const int rows = a.groups - 1;
+  if ((int)blockIdx.x < rows)
+    merge_rows<BF, true>(a, blockIdx.x);
+  else
+    merge_tiles<BF, true>(a, blockIdx.x - rows);
+}
+
 // ---------------------------------------------------------------------------
 // Host side.
 
@@ -1419,14 +1561,16 @@ __global__ void __launch_bounds__(256) fa_serve_tiles_merge_kernel(AttnArgs a) {
 constexpr int64_t kRowsMax = 64;
 
 struct Kernels {
-  const void *rows, *rows_merge, *tiles, *tiles_merge;
+  const void *rows, *tiles, *mixed, *rows_merge, *tiles_merge, *mixed_merge;
 };
 template <bool BF, bool PAGED>
 constexpr Kernels kernels_of() {
   return {reinterpret_cast<const void*>(&fa_serve_rows_kernel<BF, PAGED>),
+          reinterpret_cast<const void*>(&fa_serve_tiles_kernel<BF, PAGED, false>),
+          reinterpret_cast<const void*>(&fa_serve_tiles_kernel<BF, true, true>),
           reinterpret_cast<const void*>(&fa_serve_rows_merge_kernel<BF, PAGED>),
-          reinterpret_cast<const void*>(&fa_serve_tiles_kernel<BF, PAGED>),
-          reinterpret_cast<const void*>(&fa_serve_tiles_merge_kernel<BF, PAGED>)};
+          reinterpret_cast<const void*>(&fa_serve_tiles_merge_kernel<BF, PAGED>),
+          reinterpret_cast<const void*>(&fa_serve_mixed_merge_kernel<BF>)};
 }
 const Kernels kKernels[2][2] = {{kernels_of<false, false>(), kernels_of<false, true>()},
                                 {kernels_of<true, false>(), kernels_of<true, true>()}};
@@ -1441,8 +1585,9 @@ int ensure_lds_limits() {
   if (known && done[dev].load(std::memory_order_acquire)) return FA_SERVE_OK;
   for (const auto& type : kKernels)
     for (const Kernels& k : type) {
-      if (hipFuncSetAttribute(k.rows, hipFuncAttributeMaxDynamicSharedMemorySize, kRowsLds) != hipSuccess ||
-          hipFuncSetAttribute(k.tiles, hipFuncAttributeMaxDynamicSharedMemorySize, kTileLds) != hipSuccess)
+      if (hipFuncSetAttribute(k.rows, hipFuncAttributeMaxDynamicSharedMemorySize, rows_lds(4)) != hipSuccess ||
+          hipFuncSetAttribute(k.tiles, hipFuncAttributeMaxDynamicSharedMemorySize, kTileLds) != hipSuccess ||
+          hipFuncSetAttribute(k.mixed, hipFuncAttributeMaxDynamicSharedMemorySize, kTileLds) != hipSuccess)
         return FA_SERVE_ERR_LAUNCH;
     }
   if (known) done[dev].store(true, std::memory_order_release);
@@ -1454,6 +1599,7 @@ struct LaunchPlan {
   bool rows = false, tiles = false, split = false;
   int rows_max = 0;                         // for the kernels: see AttnArgs
   int64_t tiles_max = 0;                    // tiles, if the requests are all consistent
+  int length = kUncut;
   uint64_t opart = 0, lpart = 0, desc = 0, topart = 0, tlpart = 0, tdesc = 0, end = 0;   // offsets
 };
 LaunchPlan launch_plan(int64_t batch, int64_t heads_kv, int64_t group, int64_t tokens, int64_t max_new, bool even) {
@@ -1513,22 +1659,24 @@ int run(const AttnArgs& filled, const LaunchPlan& lp, int32_t type, bool paged, 
   a.tdesc = reinterpret_cast<int*>(ws + lp.tdesc);
   a.rows_max = lp.rows_max;
   a.split = lp.split;
-  a.groups = kRowsGroups;
+  a.length = lp.length;
+  a.groups = !lp.rows ? 0 : lp.tiles ? kRowsGroups / 2 : kRowsGroups;
   const Kernels& k = kKernels[type == FA_SERVE_BF16][paged];
   void* args[] = {&a};
   if (lp.tiles) {
     // A workgroup for every item there can be: each die's share of whole tiles
     // rounds up once a request and head.
     const int64_t h = std::min<int64_t>(a.heads_kv & -(int64_t)a.heads_kv, 8);
-    int64_t grid = 8 * (lp.tiles_max / 8 + a.heads_kv / h * a.batch + 1);
-    grid = std::max<int64_t>(grid, lp.split ? kTileItems : 8);
-    rc = enqueue(k.tiles, dim3((unsigned)grid), dim3(TTHREADS), args, kTileLds, stream);
-    if (!rc && lp.split) rc = enqueue(k.tiles_merge, dim3(kTileGroups * 32), dim3(256), args, 0, stream);
+    const int64_t grid = 8 * (lp.tiles_max / 8 + a.heads_kv / h * a.batch + 1);
+    a.tile_groups = (int)std::max<int64_t>(grid, lp.split ? kTileItems : 8);
+    rc = enqueue(lp.rows ? k.mixed : k.tiles, dim3((unsigned)(a.tile_groups + a.groups)), dim3(TTHREADS), args,
+                 kTileLds, stream);
+  } else {
+    rc = enqueue(k.rows, dim3(a.groups), dim3(256), args, rows_lds(4), stream);
   }
-  if (!rc && lp.rows) {
-    rc = enqueue(k.rows, dim3(kRowsGroups), dim3(RTHREADS), args, kRowsLds, stream);
-    if (!rc) rc = enqueue(k.rows_merge, dim3(kRowsGroups - 1), dim3(256), args, 0, stream);
-  }
+  const unsigned joins = (a.groups ? a.groups - 1 : 0) + (lp.split ? kTileGroups * 32 : 0);
+  if (!rc && joins)
+    rc = enqueue(!lp.tiles ? k.rows_merge : lp.rows ? k.mixed_merge : k.tiles_merge, dim3(joins), dim3(256), args, 0, stream);
   return rc;
 }
 
@@ -1562,6 +1710,25 @@ int check_paged(const fa_paged* p, LaunchPlan* lp) {
   return check_work(*lp, p->batch, p->heads_kv, p->heads_q / p->heads_kv, p->tokens, p->max_pages * p->page_size);
 }
 
+AttnArgs mask_args(int64_t window, int64_t sinks, float scale) {
+  AttnArgs a{};
+  a.window = window ? (int)std::min<int64_t>(window, NO_WINDOW) : NO_WINDOW;
+  a.sinks = (int)std::min<int64_t>(sinks, NO_WINDOW);
+  a.c = (float)((double)scale * LOG2E);
+  return a;
+}
+
+AttnArgs window_args(const fa_window* p) {
+  AttnArgs a = mask_args(p->window, p->sinks, p->scale);
+  a.batch = (int)p->batch;
+  a.heads_kv = (int)p->heads_kv;
+  a.group = (int)(p->heads_q / p->heads_kv);
+  a.seq_q = (int)p->seq_q;
+  a.seq_k = (int)p->seq_k;
+  a.off = p->causal == FA_WINDOW_BOTTOM_RIGHT ? (int)(p->seq_k - p->seq_q) : 0;
+  return a;
+}
+
 int check_window(const fa_window* p, LaunchPlan* lp) {
   if (!p) return FA_SERVE_ERR_NULL;
   const int64_t limit = (int64_t)1 << 30;
@@ -1576,15 +1743,22 @@ int check_window(const fa_window* p, LaunchPlan* lp) {
   if (!rc && p->causal != FA_WINDOW_TOP_LEFT && p->causal != FA_WINDOW_BOTTOM_RIGHT) rc = FA_SERVE_ERR_CAUSAL;
   if (rc) return rc;
   *lp = launch_plan(p->batch, p->heads_kv, p->heads_q / p->heads_kv, p->batch * p->seq_q, p->seq_q, true);
+  if (lp->split) {
+    const AttnArgs a = window_args(p);
+    const int longest = tile_blocks(a, request<false>(a, 0));
+    float least = 0.f;
+    for (int cut = 1; cut <= kCuts; ++cut) {
+      const int n = cut_length(cut, longest);
+      const float cost = cut_cost(cut, longest, n, lp->tiles_max * ((longest + n - 1) / n));
+      if (cut == 1 || cost < least) {
+        least = cost;
+        lp->length = cut == 1 ? kUncut : n;
+      }
+    }
+    lp->split = lp->length < kUncut;
+    if (!lp->split) lp->end = lp->topart;   // nothing but the parts is behind them
+  }
   return check_work(*lp, p->batch, p->heads_kv, p->heads_q / p->heads_kv, p->batch * p->seq_q, p->seq_k);
-}
-
-AttnArgs mask_args(int64_t window, int64_t sinks, float scale) {
-  AttnArgs a{};
-  a.window = window ? (int)std::min<int64_t>(window, NO_WINDOW) : NO_WINDOW;
-  a.sinks = (int)std::min<int64_t>(sinks, NO_WINDOW);
-  a.c = (float)((double)scale * LOG2E);
-  return a;
 }
 
 }  // namespace
@@ -1679,7 +1853,7 @@ int fa_window_fwd(const fa_window* p, const void* q, const void* k, const void* 
     if (!aligned(ptr, 16)) return FA_SERVE_ERR_ALIGN;
   if (!aligned(lse, 4)) return FA_SERVE_ERR_ALIGN;
   if ((lp.end && !workspace) || workspace_bytes < lp.end) return FA_SERVE_ERR_WORKSPACE;
-  AttnArgs a = mask_args(p->window, p->sinks, p->scale);
+  AttnArgs a = window_args(p);
   a.q = static_cast<const char*>(q);
   a.k = static_cast<const char*>(k);
   a.v = static_cast<const char*>(v);
@@ -1700,12 +1874,6 @@ int fa_window_fwd(const fa_window* p, const void* q, const void* k, const void* 
   a.ls_b = p->heads_q * p->seq_q;
   a.ls_h = p->seq_q;
   a.ls_n = 1;
-  a.batch = (int)p->batch;
-  a.heads_kv = (int)p->heads_kv;
-  a.group = (int)(p->heads_q / p->heads_kv);
-  a.seq_q = (int)p->seq_q;
-  a.seq_k = (int)p->seq_k;
-  a.off = p->causal == FA_WINDOW_BOTTOM_RIGHT ? (int)(p->seq_k - p->seq_q) : 0;
   return run(a, lp, p->type, false, workspace, stream);
 }
 
