@@ -883,9 +883,8 @@ __device__ __forceinline__ void merge_rows(const AttnArgs& a, int block) {
 // softmax step (S(j) into P(j)), so that on every SIMD one wave feeds the matrix
 // pipe while the other does its softmax; the phases are separated by barriers. LDS
 // holds two K and two V blocks of 128 keys, 256-byte rows placed as in the row
-// kernel. During its softmax of block j group 1 loads K(j + 2) and V(j + 1)
-// into the slots that were read last in the MFMA steps before; their page numbers
-// were fetched (scalar loads) a step earlier.
+// kernel. Group 1 loads the K blocks, group 0 the V blocks; their page numbers are
+// fetched (scalar loads) a step earlier.
 //
 // The blocks that every row of the tile sees whole come first, in a loop without
 // mask code, then the others: the order of keys is free in the online softmax.
@@ -983,44 +982,42 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk) qf[kk] = *reinterpret_cast<const h8*>(qrow + (kk * 2 + hf) * 16);
 
-  // Loads: group 1's wave dw fills rows 32 dw .. + 31 of a block, two 16-key groups
-  // and so two descriptors for its 8 instructions of 4 rows each.
-  int koff[4];
+  // Loads: wave dw of group 1 fills rows 32 dw .. + 31 of the K blocks, that of group 0
+  // those of the V blocks: two 16-key groups, and so two descriptors for the 8
+  // instructions of 4 rows each. The descriptor of the next load is made after a load.
+  const char* const lbase = grp ? st.k : st.v;
+  const uint32_t lpage = grp ? st.ks_b : st.vs_b;
+  const int lpitch = grp ? st.ks_n : st.vs_n;
+  int loff[4];
 #pragma unroll
-  for (int x = 0; x < 4; ++x) koff[x] = lr * st.ks_n + ((lane & 15) ^ (4 * x + lr)) * 16;
-  const int voff = lr * st.vs_n + ((lane & 15) ^ (4 * lr)) * 16;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds + dw * (32 * ROW_BYTES);
+  for (int x = 0; x < 4; ++x) loff[x] = lr * lpitch + ((lane & 15) ^ (grp ? 4 * x + lr : 4 * lr)) * 16;
+  const uint32_t ldst = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds + dw * (32 * ROW_BYTES) +
+                        (grp ? 0 : 2 * TBLOCK);
   bool bad = r.bad;
-  // First keys (of this wave) and pages of the next K block to load, of the V block to
-  // load beside it and of the K block after.
-  int kid[2], vid[2], nid[2], kkey = 0, vkey = 0, nkey = 0;
+  int id[2], key = 0, nid[2], nkey = 0;     // pages and first key (this wave's) of the next block to load, and the one after
+  i32x4 rs;
   auto fetch = [&](int s) {
     nkey = s < nblk ? block_at(s) * BLOCK + 32 * dw : 1 << 30;
 #pragma unroll
     for (int g = 0; g < 2; ++g) nid[g] = uniform(st.page(nkey + 16 * g));
   };
-  auto shift_ids = [&]() {
-    vkey = kkey;
-    kkey = nkey;
+  auto describe = [&](int g) {
+    bad |= st.missing(key + 16 * g, id[g]);
+    rs = st.rsrc(lbase, lpage, lpitch, key + 16 * g, id[g]);
+  };
+  auto advance = [&]() {                    // what was fetched is next
+    key = nkey;
+    id[0] = nid[0];
+    id[1] = nid[1];
+    describe(0);
+  };
+  auto load = [&](int x, int slot) {
+    dma_to_lds_late(rs, ldst + slot * TBLOCK + x * 1024, loff[x & 3], 4 * (x & 3) * lpitch);
+    if (x == 3) describe(1);
+  };
+  auto load_all = [&](int slot) {
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      vid[g] = kid[g];
-      kid[g] = nid[g];
-    }
-  };
-  i32x4 rs;                                 // of the group that is being loaded
-  auto load_k = [&](int x, int slot) {
-    const int g = x >> 2;
-    if ((x & 3) == 0) {
-      bad |= st.missing(kkey + 16 * g, kid[g]);
-      rs = st.k_rsrc(kkey + 16 * g, kid[g]);
-    }
-    dma_to_lds_late(rs, lds0 + slot * TBLOCK + x * 1024, koff[x & 3], 4 * (x & 3) * st.ks_n);
-  };
-  auto load_v = [&](int x, int slot) {
-    const int g = x >> 2;
-    if ((x & 3) == 0) rs = st.v_rsrc(vkey + 16 * g, vid[g]);
-    dma_to_lds_late(rs, lds0 + (2 + slot) * TBLOCK + x * 1024, voff, 4 * (x & 3) * st.vs_n);
+    for (int x = 0; x < 8; ++x) load(x, slot);
   };
 
   f32x16 acc[4], s[4];
@@ -1054,7 +1051,8 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
 #pragma unroll
     for (int x = 0; x < PF; ++x) fr[x] = ld(kb, vb, operand(decltype(kind)::value, x));
   };
-  auto mfma_step = [&](const char* kb, const char* vb, auto preloaded, auto kind) {
+  // load_at(x) runs after product N / 8 * x + 1 of the step, 0 <= x < 8.
+  auto mfma_step = [&](const char* kb, const char* vb, auto preloaded, auto kind, auto&& load_at) {
     constexpr int KIND = decltype(kind)::value;
     constexpr int N = KIND == BOTH ? 64 : 32;
     if constexpr (!decltype(preloaded)::value) preload(kb, vb, kind);
@@ -1067,6 +1065,7 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
       else
         acc[n % 4] = mma<BF>(f, p[n / 4], acc[n % 4]);
       if (x + PF < N) fr[x % PF] = ld(kb, vb, operand(KIND, x + PF));
+      if (x % (N / 8) == 1) load_at(x / (N / 8));
       __builtin_amdgcn_sched_barrier(0);    // operand reads stay PF products ahead
     }
   };
@@ -1088,18 +1087,21 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
 
   // Phase 2j + grp is a wave's MFMA step for block j, phase 2j + grp + 1 its
   // softmax; all waves pass the same 2 nblk + 3 barriers. K(j) and V(j) are in
-  // slots j % 2. Group 1 loads K(0) before the first barrier, K(1) and V(0) in
-  // phase 0 and K(j + 2), V(j + 1) in phase 2j + 2, and waits for them at the
-  // end of the next phase, before the barrier that publishes them.
+  // slots j % 2. Group 1 loads K(0) before the first barrier, K(1) in phase 0 and
+  // K(j + 2) in phase 2j + 2, its softmax, into the slot of K(j), which both groups'
+  // MFMA steps j have read. Group 0 loads V(j) in phase 2j, its MFMA step, into the
+  // slot of V(j - 2), which was last read in phase 2j - 1. A group waits for its loads
+  // at the end of the next phase, before the barrier that publishes them.
+  // (All loads in group 1's softmax made that step the longest of a phase.)
   if (tid == 0) *flag = 0;
   const bool idle = row0 >= rows;           // this wave has no row: it loads and waits only
+  auto nothing = [](int) {};
+  fetch(0);
+  advance();
   if (grp == 1) {
-    fetch(0);
-    shift_ids();
-#pragma unroll
-    for (int x = 0; x < 8; ++x) load_k(x, 0);
+    load_all(0);
     fetch(1);
-    shift_ids();
+    advance();
     wait_loads<0>();
   }
   // The compiler waits for its own loads here, before the key loop.
@@ -1108,12 +1110,24 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
   lds_barrier();
   if (grp == 0) {
     if (idle) {
-      for (int j = 0; j < 2 * nblk + 2; ++j) lds_barrier();
+      for (int j = 0; j < nblk; ++j) {
+        load_all(j & 1);
+        fetch(j + 1);
+        lds_barrier();
+        wait_loads<0>();
+        advance();
+        lds_barrier();
+      }
+      lds_barrier();
+      lds_barrier();
     } else {
       auto step = [&](int j, auto kind, auto mask) {
-        mfma_step(kslot(j), vslot(j + 1), loads, kind);
+        mfma_step(kslot(j), vslot(j + 1), loads, kind, [&](int x) { load(x, j & 1); });
         lds_barrier();
-        softmax(j, mask, [](int) {});
+        fetch(j + 1);
+        softmax(j, mask, nothing);
+        wait_loads<0>();
+        advance();
         lds_barrier();
       };
       if (nfull > 0)
@@ -1123,29 +1137,22 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
       int j = 1;
       for (; j < nfull; ++j) step(j, both, whole);
       for (; j < nblk; ++j) step(j, both, with_mask);
-      mfma_step(kslot(nblk), vslot(nblk + 1), loads, pv);
+      mfma_step(kslot(nblk), vslot(nblk + 1), loads, pv, nothing);
       lds_barrier();
       lds_barrier();
     }
   } else {
-    // Phase 0: the loads of K(1) and V(0).
-#pragma unroll
-    for (int x = 0; x < 8; ++x) load_k(x, 1);
-#pragma unroll
-    for (int x = 0; x < 8; ++x) load_v(x, 0);
+    load_all(1);                            // phase 0
     fetch(2);
-    shift_ids();
+    advance();
     if (idle) {
       lds_barrier();
       for (int j = 0; j < nblk; ++j) {
         wait_loads<0>();
         lds_barrier();
+        load_all(j & 1);
         fetch(j + 3);
-#pragma unroll
-        for (int x = 0; x < 8; ++x) load_k(x, j & 1);
-#pragma unroll
-        for (int x = 0; x < 8; ++x) load_v(x, (j + 1) & 1);
-        shift_ids();
+        advance();
         lds_barrier();
       }
       wait_loads<0>();
@@ -1154,21 +1161,17 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
       preload(kslot(0), vslot(0), qk);
       lds_barrier();
       auto step = [&](int j, auto kind, auto mask) {
-        mfma_step(kslot(j), vslot(j + 1), preloaded, kind);
+        mfma_step(kslot(j), vslot(j + 1), preloaded, kind, nothing);
         wait_loads<0>();
         lds_barrier();
         fetch(j + 3);
-        // 16 loads over the 32 pairs of exponentials.
-        softmax(j, mask, [&](int x) {
-          if (x & 1) return;
+        softmax(j, mask, [&](int x) {       // 8 loads over the 32 pairs of exponentials
+          if (x % 4) return;
           __builtin_amdgcn_sched_barrier(0);
-          if (x < 16)
-            load_k(x / 2, j & 1);
-          else
-            load_v(x / 2 - 8, (j + 1) & 1);
+          load(x / 4, j & 1);
           __builtin_amdgcn_sched_barrier(0);
         });
-        shift_ids();
+        advance();
         preload(kslot(j + 1), vslot(j), both);
         lds_barrier();
       };
@@ -1179,12 +1182,12 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
       int j = 1;
       for (; j < nfull; ++j) step(j, both, whole);
       for (; j < nblk; ++j) step(j, both, with_mask);
-      mfma_step(kslot(nblk), vslot(nblk + 1), loads, pv);
+      mfma_step(kslot(nblk), vslot(nblk + 1), loads, pv, nothing);
       wait_loads<0>();
       lds_barrier();
     }
-    if (bad && lane == 0) *flag = 1;
   }
+  if (bad && lane == 0) *flag = 1;
   lds_barrier();                            // nobody reads the ring any more; flag is set
   const bool poisoned = *flag != 0 || r.bad;
 
