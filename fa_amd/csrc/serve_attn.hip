@@ -118,8 +118,7 @@ __device__ __forceinline__ uint32_t lanes_sum(uint32_t x) {
 // A batch entry: the first of its rows in q, their number, the position of
 // row 0, its keys, and whether its table row is too short for them.
 struct Request {
-  int row0, n, pos, keys;
-  bool bad;
+  int row0, n, pos, keys, bad;
 };
 template <bool PAGED>
 __host__ __device__ __forceinline__ Request request(const AttnArgs& a, int b) {
@@ -138,24 +137,15 @@ __host__ __device__ __forceinline__ Request request(const AttnArgs& a, int b) {
     r.n = a.seq_q;
     r.pos = a.off;
     r.keys = a.seq_k;
-    r.bad = false;
+    r.bad = 0;
   }
   return r;
 }
 
 // The request of a whole workgroup, in scalar registers: descriptors and loop
 // bounds are made from it.
-template <bool PAGED>
-__device__ __forceinline__ Request uniform_request(const AttnArgs& a, int b) {
-  Request r = request<PAGED>(a, b);
-  if constexpr (PAGED) {
-    r.row0 = __builtin_amdgcn_readfirstlane(r.row0);
-    r.n = __builtin_amdgcn_readfirstlane(r.n);
-    r.pos = __builtin_amdgcn_readfirstlane(r.pos);
-    r.keys = __builtin_amdgcn_readfirstlane(r.keys);
-    r.bad = __builtin_amdgcn_readfirstlane((int)r.bad);
-  }
-  return r;
+__device__ __forceinline__ Request uniform(const Request& r) {
+  return Request{uniform(r.row0), uniform(r.n), uniform(r.pos), uniform(r.keys), uniform(r.bad)};
 }
 
 // The key blocks that rows at positions first .. last see: blocks [0, ns) and
@@ -666,8 +656,9 @@ template <bool BF, bool PAGED, int RW>
 __device__ __forceinline__ void rows_share(const AttnArgs& a, int g, char* lds) {
   constexpr int RTHREADS = RW * 64;
   __shared__ float st_m[RW * RT], st_l[RW * RT];
-  __shared__ uint32_t wave_sum[RW];
+  __shared__ uint32_t wave_sum[RW][2];
   __shared__ int found[2];
+  __shared__ Request found_r;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   // Blocks of all items before this thread's run of requests, and of all.
   const int per = (a.batch + RTHREADS - 1) / RTHREADS;
@@ -676,16 +667,25 @@ __device__ __forceinline__ void rows_share(const AttnArgs& a, int g, char* lds) 
     const int tiles = row_tiles<PAGED>(a, r);
     return tiles ? (uint32_t)(a.heads_kv * tiles * row_blocks(a, r)) : 0u;
   };
-  uint32_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += cost(request<PAGED>(a, b));
-  const uint32_t sum = lanes_sum(mine);
-  if (lane == 63) wave_sum[wave] = sum;
+  Request own{};                            // of request b0
+  uint64_t all = 0;
+  for (int b = b0; b < b1; ++b) {
+    const Request r = request<PAGED>(a, b);
+    if (b == b0) own = r;
+    all += cost(r);
+  }
+  const uint32_t mine = (uint32_t)all, sum = lanes_sum(mine), upper = lanes_sum((uint32_t)(all >> 16));
+  if (lane == 63) {
+    wave_sum[wave][0] = sum;
+    wave_sum[wave][1] = upper;
+  }
   __syncthreads();
-  uint32_t before = sum - mine, total = 0;
+  uint32_t before = sum - mine, total = 0, large = 0;
 #pragma unroll
   for (int w = 0; w < RW; ++w) {
-    if (w < wave) before += wave_sum[w];
-    total += wave_sum[w];
+    if (w < wave) before += wave_sum[w][0];
+    total += wave_sum[w][0];
+    large += wave_sum[w][1];
   }
   total = uniform(total);
   const uint32_t share = max(uniform((total + a.groups - 1) / a.groups), (uint32_t)kMinShare);
@@ -693,26 +693,28 @@ __device__ __forceinline__ void rows_share(const AttnArgs& a, int g, char* lds) 
   const uint32_t end = min(x + share, total);
   int* desc = a.desc + g * DESC_INTS;
   if (tid == 0) desc[3] = -1;               // no item that began earlier, so far
-  if (x >= total) return;                   // uniform
-  if (tid == 0) found[0] = a.batch;
-  __syncthreads();
+  // Uniform. (`large`: requests that overlap, beyond what 32 bits count.)
+  if (x >= total || large >= 1 << 15) return;
   if (before <= x && x < before + mine) {
     int b = b0;
     uint32_t at = before;
-    for (;; ++b) {
-      const uint32_t n = cost(request<PAGED>(a, b));
-      if (x < at + n) break;
+    Request r = own;
+    while (true) {
+      const uint32_t n = cost(r);
+      if (x < at + n || b + 1 >= b1) break;
       at += n;
+      r = request<PAGED>(a, ++b);
     }
     found[0] = b;
     found[1] = (int)at;
+    found_r = r;
   }
   __syncthreads();
-  int b = __builtin_amdgcn_readfirstlane(found[0]);
+  int b = uniform(found[0]);
   uint32_t at = uniform((uint32_t)found[1]);          // where request b's blocks start
+  Request r = uniform(found_r);
   bool head = true;
-  for (; b < a.batch; ++b) {
-    const Request r = uniform_request<PAGED>(a, b);
+  while (true) {
     const int tiles = row_tiles<PAGED>(a, r);
     if (tiles) {
       const int nblk = uniform(row_blocks(a, r));
@@ -723,13 +725,15 @@ __device__ __forceinline__ void rows_share(const AttnArgs& a, int g, char* lds) 
         const int s1 = uniform((int)min((uint32_t)nblk, s0 + (end - x)));
         const int hk = uniform((int)(item / (uint32_t)tiles)), tile = uniform((int)(item - (uint32_t)hk * tiles));
         if (head && s0 > 0 && tid == 0) {
-          // The workgroups that share an item that began before this one's share.
+          // An item that began before this one's share: what the merge kernel needs.
           const uint32_t start = x - s0;
           desc[0] = b;
           desc[1] = hk;
           desc[2] = tile;
-          desc[3] = (int)(start / share);
+          desc[3] = (int)(start / share);   // the workgroups that share it
           desc[4] = (int)((start + nblk - 1) / share);
+          desc[5] = r.row0;
+          desc[6] = r.n * a.group;
         }
         head = false;
         row_item<BF, PAGED, RW>(a, r, b, hk, tile, s0, s1, nblk, 2 * g + (s0 == 0), lds, st_m, st_l);
@@ -738,6 +742,8 @@ __device__ __forceinline__ void rows_share(const AttnArgs& a, int g, char* lds) 
       at = stop;
     }
     if (x >= end) break;
+    if (++b >= a.batch) break;
+    r = uniform(request<PAGED>(a, b));
   }
 }
 
@@ -767,32 +773,33 @@ __device__ __forceinline__ void merge_rows(const AttnArgs& a, int block) {
   const int* desc = a.desc + (block + 1) * DESC_INTS;
   const int first = desc[3];
   if (first < 0) return;
-  const int b = desc[0], hk = desc[1], tile = desc[2], last = desc[4];
+  const int b = desc[0], hk = desc[1], tile = desc[2], last = desc[4], row0 = desc[5];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int boundaries = last - first, pieces = boundaries + 1, mine = block - first;
-  const Request r = request<PAGED>(a, b);
-  const int rows = min(r.n * a.group - tile * RT, RT);
-  auto piece = [&](int s) { return (int64_t)(2 * (first + s) + (s == 0)); };
-  auto row_of = [&](int n, int& i, int& head) {
-    const int row = tile * RT + n;
-    i = row / a.group;
-    head = hk * a.group + row % a.group;
-  };
+  const int rows = min(desc[6] - tile * RT, RT);
+  auto piece = [&](int s) { return 2 * (first + s) + (s == 0); };
   auto out_row = [&](int n) {
-    int i, head;
-    row_of(n, i, head);
-    return a.o + b * a.os_b + (int64_t)(r.row0 + i) * a.os_n + head * a.os_h;
+    const int row = tile * RT + n, i = row / a.group, head = hk * a.group + row % a.group;
+    return a.o + b * a.os_b + (int64_t)(row0 + i) * a.os_n + head * a.os_h;
   };
   auto out_lse = [&](int n, float M, float total) {
     if (!a.lse) return;
-    int i, head;
-    row_of(n, i, head);
-    a.lse[b * a.ls_b + (int64_t)(r.row0 + i) * a.ls_n + head * a.ls_h] = M == -INFINITY ? M : M + logf(total);
+    const int row = tile * RT + n, i = row / a.group, head = hk * a.group + row % a.group;
+    a.lse[b * a.ls_b + (int64_t)(row0 + i) * a.ls_n + head * a.ls_h] = M == -INFINITY ? M : M + logf(total);
   };
   if (pieces <= kFewPieces) {
     const int l32 = tid & 31;
     for (int n = mine + (tid >> 5) * boundaries; n < rows; n += 8 * boundaries) {
+      // The first pieces' rows beside their lse: past the last piece, that one
+      // again with weight 0.
+      float4 v[8];
+      auto read = [&](int s0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          v[e] = *reinterpret_cast<const float4*>(a.opart + (piece(min(s0 + e, boundaries)) * RT + n) * HD + 4 * l32);
+      };
       const float x = l32 < pieces ? a.lpart[piece(l32) * RT + n] : -INFINITY;
+      read(0);
       float M = x;
 #pragma unroll
       for (int d = 16; d >= 1; d >>= 1) M = smax(M, __shfl_xor(M, d, 32));
@@ -802,10 +809,7 @@ __device__ __forceinline__ void merge_rows(const AttnArgs& a, int block) {
       for (int d = 16; d >= 1; d >>= 1) total += __shfl_xor(total, d, 32);
       float4 o = {0.f, 0.f, 0.f, 0.f};
       for (int s0 = 0; s0 < pieces; s0 += 8) {
-        float4 v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e)         // past the last piece: that one again, weight 0
-          v[e] = *reinterpret_cast<const float4*>(a.opart + (piece(min(s0 + e, pieces - 1)) * RT + n) * HD + 4 * l32);
+        if (s0) read(s0);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float ws = __shfl(w, min(s0 + e, 31), 32) * (s0 + e < pieces ? 1.f : 0.f);
@@ -1462,11 +1466,7 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, const Dies& d, uint
   it.length = uniform(it.length);
   it.index = uniform(it.index);
   it.tile_index = uniform(it.tile_index);
-  it.r.row0 = uniform(it.r.row0);
-  it.r.n = uniform(it.r.n);
-  it.r.pos = uniform(it.r.pos);
-  it.r.keys = uniform(it.r.keys);
-  it.r.bad = uniform((int)it.r.bad);
+  it.r = uniform(it.r);
   return true;
 }
 

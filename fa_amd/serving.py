@@ -143,47 +143,41 @@ class _Operator:
     def __init__(self, library):
         self.lib = library if isinstance(library, C.CDLL) else load_library(library)
         self.plans = {}
+        self.streams = {}        # (device index, raw stream) -> torch stream
 
     def check(self, status, where):
         if status:
             raise RuntimeError(f"{where}: {status} ({self.lib.fa_serve_strerror(status).decode()})")
 
-    def planned(self, key, make):
-        plan = self.plans.get(key)
-        if plan is None:
-            plan = make()
-            if len(self.plans) >= SIGNATURES_KEPT:
-                self.plans.clear()
-            self.plans[key] = plan
+    def keep(self, key, plan):
+        if len(self.plans) >= SIGNATURES_KEPT:
+            self.plans.clear()
+        self.plans[key] = plan
         return plan
 
-    def launch(self, device, enqueue, where, tensors):
-        """enqueue(raw stream) with `device` current; the tensors, which may come
-        from other streams, are kept from being reused before it has run."""
+    def launch(self, fn, args, device, tensors):
+        """fn(*args, stream) with `device` current. The tensors, which may come from
+        other streams, are kept from being reused before it has run."""
         import torch
 
         index = device.index
-        if index == torch.cuda.current_device():
-            status = enqueue(torch._C._cuda_getCurrentRawStream(index))
-        else:
+        if index != torch.cuda.current_device():
             with torch.cuda.device(index):
-                status = enqueue(torch._C._cuda_getCurrentRawStream(index))
+                return self.launch(fn, args, device, tensors)
+        raw = torch._C._cuda_getCurrentRawStream(index)
+        stream = self.streams.get((index, raw))
+        if stream is None:
+            if len(self.streams) >= 64:
+                self.streams.clear()
+            stream = self.streams[index, raw] = torch.cuda.current_stream(index)
+        status = fn(*args, raw)
         if status:
-            self.check(status, where)
-        stream = torch.cuda.current_stream(index)
+            self.check(status, fn.__name__)
         for t in tensors:
             t.record_stream(stream)
 
-    def workspace(self, size, device):
-        import torch
 
-        return torch.empty(size, dtype=torch.uint8, device=device) if size else None
-
-
-def _aligned(*tensors):
-    for t in tensors:
-        if t.data_ptr() % 16:
-            raise ValueError(f"rows of {DIM} dims must be 16-byte aligned")
+ALIGN_ERROR = f"rows of {DIM} dims must be 16-byte aligned"
 
 
 class PagePlanner(_Operator):
@@ -214,23 +208,25 @@ class PagePlanner(_Operator):
     def __call__(self, past, new, table, pages, taken, tokens):
         import torch
 
-        key = (_signature(past), _signature(new), _signature(table), _signature(pages),
-               _signature(taken), tokens)
-        prob = self.planned(key, lambda: self.plan(past, new, table, pages, taken, tokens))
-        device, batch = past.device, past.shape[0]
-        # One allocation: taken, lengths, starts, positions, slots.
-        sizes = (1, batch, batch + 1, tokens, tokens)
-        made = torch.empty(sum(sizes), dtype=torch.int32, device=device).split(sizes)
-        taken_out, lengths, starts, positions, slots = made
-
-        def enqueue(stream):
-            return self.lib.fa_plan_pages(
-                prob, past.data_ptr(), new.data_ptr(), table.data_ptr(), pages.data_ptr(),
-                taken.data_ptr(), starts.data_ptr(), lengths.data_ptr(), positions.data_ptr(),
-                slots.data_ptr(), taken_out.data_ptr(), stream)
-
-        self.launch(device, enqueue, "fa_plan_pages", (past, new, table, pages, taken))
-        return PagePlan(starts, lengths, positions, slots, taken_out)
+        # One lookup stands for the checks of a signature met before.
+        key = (past.shape, past.stride(), past.dtype, past.device, new.shape, new.stride(),
+               new.dtype, new.device, table.shape, table.stride(), table.dtype, table.device,
+               pages.shape, pages.stride(), pages.dtype, pages.device, taken.shape, taken.stride(),
+               taken.dtype, taken.device, tokens)
+        plan = self.plans.get(key)
+        if plan is None:
+            plan = self.keep(key, self.plan(past, new, table, pages, taken, tokens))
+        prob, sizes, total = plan
+        device = past.device
+        made = torch.empty(total, dtype=torch.int32, device=device)
+        at = made.data_ptr()
+        lengths = at + 4 * sizes[0]
+        positions = lengths + 4 * sizes[1]
+        self.launch(self.lib.fa_plan_pages,
+                    (prob, past.data_ptr(), new.data_ptr(), table.data_ptr(), pages.data_ptr(),
+                     taken.data_ptr(), at, lengths, positions, positions + 4 * tokens,
+                     at + 4 * (total - 1)), device, (past, new, table, pages, taken))
+        return PagePlan(*made.split_with_sizes(sizes))
 
     def plan(self, past, new, table, pages, taken, tokens):
         if past.ndim != 1 or not 1 <= past.shape[0] <= self.MAX_BATCH:
@@ -243,8 +239,10 @@ class PagePlanner(_Operator):
         if not isinstance(tokens, int) or not 0 <= tokens <= 1 << 30:
             raise ValueError("tokens must be an int from 0 to 2^30")
         _on_gpu(past.device, new, table, pages, taken)
+        # One allocation: starts, lengths, positions, slots, taken.
+        sizes = [batch + 1, batch, tokens, tokens, 1]
         return FaPagePlan(batch, tokens, self.page_size, table.shape[1],
-                          max(table.stride(0), table.shape[1]), pages.shape[0])
+                          max(table.stride(0), table.shape[1]), pages.shape[0]), sizes, sum(sizes)
 
 
 @dataclass(frozen=True)
@@ -347,39 +345,43 @@ class Rotary(_Operator):
     def __call__(self, x, positions, backward=False, out=None):
         import torch
 
-        key = (_signature(x), _signature(positions), backward, _signature(out))
-        prob, turns = self.planned(key, lambda: self.plan(x, positions, out, backward))
+        key = (x.shape, x.stride(), x.dtype, x.device, _signature(positions), backward,
+               _signature(out))
+        plan = self.plans.get(key)
+        if plan is None:
+            plan = self.keep(key, self.plan(x, positions, out, backward))
+        prob, turns = plan
         if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        _aligned(x, out)
-
-        def enqueue(stream):
-            return self.lib.fa_rotary_append(prob, x.data_ptr(), out.data_ptr(), None, None,
-                                             positions.data_ptr(), None, turns.data_ptr(), None,
-                                             None, stream)
-
-        self.launch(x.device, enqueue, "fa_rotary_append", (x, out, positions))
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        xp, op = x.data_ptr(), out.data_ptr()
+        if (xp | op) % 16:
+            raise ValueError(ALIGN_ERROR)
+        self.launch(self.lib.fa_rotary_append,
+                    (prob, xp, op, None, None, positions.data_ptr(), None, turns.data_ptr(), None,
+                     None), x.device, (x, out, positions))
         return out
 
     def append(self, q, k, v, positions, slots, k_cache, v_cache, out=None):
         import torch
 
-        key = (_signature(q), _signature(k), _signature(v), _signature(positions),
-               _signature(slots), _signature(k_cache), _signature(v_cache), _signature(out))
-        prob, turns = self.planned(
-            key, lambda: self.plan_append(q, k, v, positions, slots, k_cache, v_cache, out))
+        key = (q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), k.dtype, k.device,
+               v.shape, v.stride(), v.dtype, v.device, positions.shape, positions.stride(),
+               positions.dtype, positions.device, slots.shape, slots.stride(), slots.dtype,
+               slots.device, k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.device,
+               v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device, _signature(out))
+        plan = self.plans.get(key)
+        if plan is None:
+            plan = self.keep(key, self.plan_append(q, k, v, positions, slots, k_cache, v_cache, out))
+        prob, turns = plan
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _aligned(q, k, v, k_cache, v_cache, out)
-
-        def enqueue(stream):
-            return self.lib.fa_rotary_append(
-                prob, q.data_ptr(), out.data_ptr(), k.data_ptr(), v.data_ptr(),
-                positions.data_ptr(), slots.data_ptr(), turns.data_ptr(), k_cache.data_ptr(),
-                v_cache.data_ptr(), stream)
-
-        self.launch(q.device, enqueue, "fa_rotary_append",
-                    (q, k, v, out, positions, slots, k_cache, v_cache))
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        qp, op, kp, vp = q.data_ptr(), out.data_ptr(), k.data_ptr(), v.data_ptr()
+        kc, vc = k_cache.data_ptr(), v_cache.data_ptr()
+        if (qp | op | kp | vp | kc | vc) % 16:
+            raise ValueError(ALIGN_ERROR)
+        self.launch(self.lib.fa_rotary_append,
+                    (prob, qp, op, kp, vp, positions.data_ptr(), slots.data_ptr(), turns.data_ptr(),
+                     kc, vc), q.device, (q, k, v, out, positions, slots, k_cache, v_cache))
         return out
 
     def plan(self, x, positions, out, backward=False):
@@ -486,24 +488,29 @@ class PagedAttention(_Operator):
                  return_lse=False, out=None):
         import torch
 
-        key = (_signature(q), _signature(k_cache), _signature(v_cache), _signature(table),
-               _signature(query_starts), _signature(key_lengths), max_new, scale, _signature(out))
-        prob, size = self.planned(key, lambda: self.plan(
-            q, k_cache, v_cache, table, query_starts, key_lengths, max_new, scale, out))
+        key = (q.shape, q.stride(), q.dtype, q.device, k_cache.shape, k_cache.stride(),
+               k_cache.dtype, k_cache.device, v_cache.shape, v_cache.stride(), v_cache.dtype,
+               v_cache.device, table.shape, table.stride(), table.dtype, table.device,
+               query_starts.shape, query_starts.stride(), query_starts.dtype, query_starts.device,
+               key_lengths.shape, key_lengths.stride(), key_lengths.dtype, key_lengths.device,
+               max_new, scale, _signature(out))
+        plan = self.plans.get(key)
+        if plan is None:
+            plan = self.keep(key, self.plan(q, k_cache, v_cache, table, query_starts, key_lengths,
+                                            max_new, scale, out))
+        prob, size = plan
         device = q.device
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         lse = torch.empty(q.shape[:2], dtype=torch.float32, device=device) if return_lse else None
-        _aligned(q, k_cache, v_cache, out)
-        ws = self.workspace(size, device)
-
-        def enqueue(stream):
-            return self.lib.fa_paged_fwd(
-                prob, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(),
-                query_starts.data_ptr(), key_lengths.data_ptr(), out.data_ptr(),
-                lse.data_ptr() if return_lse else None, ws.data_ptr() if size else None, size, stream)
-
-        self.launch(device, enqueue, "fa_paged_fwd",
+        ws = torch.empty(size, dtype=torch.uint8, device=device)
+        qp, kc, vc, op = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
+        if (qp | kc | vc | op) % 16:
+            raise ValueError(ALIGN_ERROR)
+        self.launch(self.lib.fa_paged_fwd,
+                    (prob, qp, kc, vc, table.data_ptr(), query_starts.data_ptr(),
+                     key_lengths.data_ptr(), op, lse.data_ptr() if return_lse else None,
+                     ws.data_ptr(), size), device,
                     (q, k_cache, v_cache, table, query_starts, key_lengths, out))
         return (out, lse) if return_lse else out
 
@@ -533,7 +540,7 @@ class PagedAttention(_Operator):
         prob.k_cache[:], prob.v_cache[:] = _strides(k_cache, "k_cache"), _strides(v_cache, "v_cache")
         size = C.c_uint64()
         self.check(self.lib.fa_paged_workspace_bytes(prob, C.byref(size)), "fa_paged_workspace_bytes")
-        return prob, size.value
+        return prob, max(size.value, 16)
 
 
 def _out_strides(q, out):
@@ -582,21 +589,23 @@ class WindowAttention(_Operator):
     def __call__(self, q, k, v, scale=None, return_lse=False, out=None):
         import torch
 
-        key = (_signature(q), _signature(k), _signature(v), scale, _signature(out))
-        prob, size = self.planned(key, lambda: self.plan(q, k, v, scale, out))
+        key = (q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), k.dtype, k.device,
+               v.shape, v.stride(), v.dtype, v.device, scale, _signature(out))
+        plan = self.plans.get(key)
+        if plan is None:
+            plan = self.keep(key, self.plan(q, k, v, scale, out))
+        prob, size = plan
         device = q.device
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         lse = torch.empty(q.shape[:3], dtype=torch.float32, device=device) if return_lse else None
-        _aligned(q, k, v, out)
-        ws = self.workspace(size, device)
-
-        def enqueue(stream):
-            return self.lib.fa_window_fwd(
-                prob, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                lse.data_ptr() if return_lse else None, ws.data_ptr() if size else None, size, stream)
-
-        self.launch(device, enqueue, "fa_window_fwd", (q, k, v, out))
+        ws = torch.empty(size, dtype=torch.uint8, device=device)
+        qp, kp, vp, op = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+        if (qp | kp | vp | op) % 16:
+            raise ValueError(ALIGN_ERROR)
+        self.launch(self.lib.fa_window_fwd,
+                    (prob, qp, kp, vp, op, lse.data_ptr() if return_lse else None, ws.data_ptr(),
+                     size), device, (q, k, v, out))
         return (out, lse) if return_lse else out
 
     def plan(self, q, k, v, scale, out):
@@ -616,4 +625,4 @@ class WindowAttention(_Operator):
         prob.k[:], prob.v[:] = _strides(k, "k"), _strides(v, "v")
         size = C.c_uint64()
         self.check(self.lib.fa_window_workspace_bytes(prob, C.byref(size)), "fa_window_workspace_bytes")
-        return prob, size.value
+        return prob, max(size.value, 16)
