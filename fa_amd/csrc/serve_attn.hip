@@ -688,9 +688,18 @@ __device__ __forceinline__ void rows_share(const AttnArgs& a, int g, char* lds) 
     large += wave_sum[w][1];
   }
   total = uniform(total);
-  const uint32_t share = max(uniform((total + a.groups - 1) / a.groups), (uint32_t)kMinShare);
-  uint32_t x = share * g;
-  const uint32_t end = min(x + share, total);
+  // Workgroup g takes blocks [g total / groups, (g + 1) total / groups): shares that
+  // differ by one block at most, so that every CU's two workgroups have as much.
+  const uint32_t groups = max(min((uint32_t)a.groups, (total + kMinShare - 1) / kMinShare), 1u);
+  const bool narrow = total < 1u << 22;     // products with `groups` fit 32 bits
+  auto start_of = [&](uint32_t n) {
+    return uniform(narrow ? n * total / groups : (uint32_t)((uint64_t)n * total / groups));
+  };
+  auto taker_of = [&](uint32_t block) {
+    return (int)(narrow ? ((block + 1) * groups - 1) / total : (((uint64_t)block + 1) * groups - 1) / total);
+  };
+  uint32_t x = (uint32_t)g < groups ? start_of(g) : total;
+  const uint32_t end = (uint32_t)g < groups ? start_of(g + 1) : total;
   int* desc = a.desc + g * DESC_INTS;
   if (tid == 0) desc[3] = -1;               // no item that began earlier, so far
   // Uniform. (`large`: requests that overlap, beyond what 32 bits count.)
@@ -730,8 +739,8 @@ __device__ __forceinline__ void rows_share(const AttnArgs& a, int g, char* lds) 
           desc[0] = b;
           desc[1] = hk;
           desc[2] = tile;
-          desc[3] = (int)(start / share);   // the workgroups that share it
-          desc[4] = (int)((start + nblk - 1) / share);
+          desc[3] = taker_of(start);        // the workgroups that share it
+          desc[4] = taker_of(start + nblk - 1);
           desc[5] = r.row0;
           desc[6] = r.n * a.group;
         }
