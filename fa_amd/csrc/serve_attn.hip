@@ -799,8 +799,7 @@ __device__ __forceinline__ void merge_rows(const AttnArgs& a, int block) {
   if (pieces <= kFewPieces) {
     const int l32 = tid & 31;
     for (int n = mine + (tid >> 5) * boundaries; n < rows; n += 8 * boundaries) {
-      // The first pieces' rows beside their lse: past the last piece, that one
-      // again with weight 0.
+      // The first pieces' rows beside their lse (past the last piece, that one again).
       float4 v[8];
       auto read = [&](int s0) {
 #pragma unroll
@@ -821,7 +820,8 @@ __device__ __forceinline__ void merge_rows(const AttnArgs& a, int block) {
         if (s0) read(s0);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float ws = __shfl(w, min(s0 + e, 31), 32) * (s0 + e < pieces ? 1.f : 0.f);
+          if (s0 + e >= pieces) break;      // not by a weight of 0: the last piece may hold an infinity
+          const float ws = __shfl(w, s0 + e, 32);
           o.x = __builtin_fmaf(ws, v[e].x, o.x);
           o.y = __builtin_fmaf(ws, v[e].y, o.y);
           o.z = __builtin_fmaf(ws, v[e].z, o.z);
@@ -1216,7 +1216,7 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
 #pragma unroll
     for (int x = 0; x < 16; ++x) check += acc[dt][x] * 0.f;
   const bool sick = row_ok && is_nan(check) && !is_nan(lsum);
-  uint64_t again = nfull < nblk ? __builtin_amdgcn_ballot_w64(sick) : 0;
+  uint64_t again = __builtin_amdgcn_ballot_w64(sick);
   again |= again >> 32;
   again &= 0xffffffffull;                   // a bit a row
   const uint32_t repaired = (uint32_t)again;

@@ -415,10 +415,10 @@ class Rotary(_Operator):
         if not q.dtype == k.dtype == v.dtype == k_cache.dtype == v_cache.dtype:
             raise ValueError("q, k, v and the caches must have one type")
         _ints({"slots": (tokens,)}, slots=slots)
+        strides = [_strides(t, n) for t, n in ((k, "k"), (v, "v"), (k_cache, "k_cache"), (v_cache, "v_cache"))]
         _on_gpu(q.device, k, v, slots, k_cache, v_cache)
         prob.heads_kv, prob.pages, prob.page_size = k.shape[1], k_cache.shape[0], k_cache.shape[1]
-        prob.k[:], prob.v[:] = _strides(k, "k"), _strides(v, "v")
-        prob.k_cache[:], prob.v_cache[:] = _strides(k_cache, "k_cache"), _strides(v_cache, "v_cache")
+        prob.k[:], prob.v[:], prob.k_cache[:], prob.v_cache[:] = strides
         return prob, turns
 
 
@@ -531,13 +531,14 @@ class PagedAttention(_Operator):
         kind = _type(q)
         if not q.dtype == k_cache.dtype == v_cache.dtype:
             raise ValueError("q and the caches must have one type")
+        strides = [_strides(t, n) for t, n in ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"))]
         _on_gpu(q.device, k_cache, v_cache, table, query_starts, key_lengths)
         prob = FaPaged(batch, q.shape[0], q.shape[1], k_cache.shape[2], min(max_new, 1 << 40),
                        k_cache.shape[0], k_cache.shape[1], table.shape[1],
                        max(table.stride(0), table.shape[1]), self.config.window or 0,
                        self.config.sinks, _check_scale(scale), kind)
-        prob.q[:], prob.o[:] = _strides(q, "q"), _out_strides(q, out)
-        prob.k_cache[:], prob.v_cache[:] = _strides(k_cache, "k_cache"), _strides(v_cache, "v_cache")
+        prob.q[:], prob.k_cache[:], prob.v_cache[:] = strides
+        prob.o[:] = _out_strides(q, out)
         size = C.c_uint64()
         self.check(self.lib.fa_paged_workspace_bytes(prob, C.byref(size)), "fa_paged_workspace_bytes")
         return prob, max(size.value, 16)
@@ -617,12 +618,13 @@ class WindowAttention(_Operator):
         kind = _type(q)
         if not q.dtype == k.dtype == v.dtype:
             raise ValueError("q, k and v must have one type")
+        strides = [_strides(t, n) for t, n in ((q, "q"), (k, "k"), (v, "v"))]
         _on_gpu(q.device, k, v)
         prob = FaWindow(q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2],
                         self.config.window, self.config.sinks, _check_scale(scale), kind,
                         CAUSAL[self.config.causal])
-        prob.q[:], prob.o[:] = _strides(q, "q"), _out_strides(q, out)
-        prob.k[:], prob.v[:] = _strides(k, "k"), _strides(v, "v")
+        prob.q[:], prob.k[:], prob.v[:] = strides
+        prob.o[:] = _out_strides(q, out)
         size = C.c_uint64()
         self.check(self.lib.fa_window_workspace_bytes(prob, C.byref(size)), "fa_window_workspace_bytes")
         return prob, max(size.value, 16)

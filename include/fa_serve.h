@@ -125,7 +125,8 @@ int fa_rotary_append(const fa_rotary* p, const void* q, void* q_out, const void*
  * the visible keys, query head h with KV head h / (heads_q / heads_kv); a row
  * that sees no key gets o = 0 and lse = -inf. lse [tokens, heads_q] (FP32) may
  * be NULL. What the cache holds at keys a row does not see has no influence on
- * it, NaN and infinities included.
+ * it, NaN and infinities included. Scores are FP32 and may reach 1e7 in magnitude
+ * (scale q.k); a row that sees an infinite or NaN score gets NaN.
  *
  * max_new is a bound on the new tokens of a request, known to the caller; it
  * chooses kernels only, a larger request is still computed. Rows outside
