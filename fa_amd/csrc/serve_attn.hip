@@ -990,11 +990,6 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
   }
 
   const Stream<PAGED> st(a, r, b, hk);
-  const char* qrow = a.q + b * a.qs_b + (int64_t)(r.row0 + i) * a.qs_n + head * a.qs_h;
-  h8 qf[8];
-#pragma unroll
-  for (int kk = 0; kk < 8; ++kk) qf[kk] = *reinterpret_cast<const h8*>(qrow + (kk * 2 + hf) * 16);
-
   // Loads: wave dw of group 1 fills rows 32 dw .. + 31 of the K blocks, that of group 0
   // those of the V blocks: two 16-key groups, and so two descriptors for the 8
   // instructions of 4 rows each. The descriptor of the next load is made after a load.
@@ -1033,6 +1028,7 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
     for (int x = 0; x < 8; ++x) load(x, slot);
   };
 
+  h8 qf[8];
   f32x16 acc[4], s[4];
   h8 p[8];
 #pragma unroll
@@ -1111,8 +1107,11 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
   auto nothing = [](int) {};
   fetch(0);
   advance();
+  if (grp == 1) load_all(0);
+  const char* qrow = a.q + b * a.qs_b + (int64_t)(r.row0 + i) * a.qs_n + head * a.qs_h;
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) qf[kk] = *reinterpret_cast<const h8*>(qrow + (kk * 2 + hf) * 16);
   if (grp == 1) {
-    load_all(0);
     fetch(1);
     advance();
     wait_loads<0>();
@@ -1307,24 +1306,16 @@ struct Dies {
   }
   __device__ __forceinline__ int items_of(int b, int tiles) const { return heads_kv / h * tiles_of(b, tiles); }
   // The rel-th of these.
-  __device__ __forceinline__ void whole(int b, int tiles, int rel, Item& it) const {
+  __device__ __forceinline__ Item whole(const Request& r, int b, int tiles, int rel) const {
     const int here = tiles_of(b, tiles), unit = rel / here;
-    it.b = b;
-    it.hk = unit * h + die % h;
-    it.tile = tiles - 1 - (first(b) + (rel - unit * here) * step);
-    it.part = it.index = it.tile_index = 0;
-    it.parts = 1;
+    return Item{b, unit * h + die % h, tiles - 1 - (first(b) + (rel - unit * here) * step), 0, 1, kUncut, 0, 0, r};
   }
   // The rel-th part of request b, whose parts and tiles others precede.
-  __device__ __forceinline__ void part(int b, int tiles, int parts, int rel, int before, int tiles_before, Item& it) const {
-    const int unit = rel / tiles;
-    it.b = b;
-    it.hk = unit / parts;
-    it.part = unit - it.hk * parts;
-    it.tile = tiles - 1 - (rel - unit * tiles);
-    it.parts = parts;
-    it.tile_index = tiles_before + it.hk * tiles + it.tile;
-    it.index = before + (it.hk * tiles + it.tile) * parts + it.part;
+  __device__ __forceinline__ Item part(const Request& r, int b, int tiles, int parts, int length, int rel, int before,
+                                       int tiles_before) const {
+    const int unit = rel / tiles, hk = unit / parts, at = unit - hk * parts;
+    const int tile = tiles - 1 - (rel - unit * tiles), place = hk * tiles + tile;
+    return Item{b, hk, tile, at, parts, length, before + place * parts + at, tiles_before + place, r};
   }
   // This die's part number `slot` of `total`; total if it has no such part.
   __device__ __forceinline__ uint32_t eighth(uint32_t slot, uint32_t total) const {
@@ -1333,29 +1324,27 @@ struct Dies {
   }
 };
 
-// The item of workgroup `slot` of its die, if it has one. Contiguous: every request
-// is alike, and the host has chosen the cut.
+// The item of workgroup `slot` of its die; b < 0 if it has none. Contiguous: every
+// request is alike, and the host has chosen the cut.
 template <bool BF, bool PAGED>
-__device__ __forceinline__ bool find_item(const AttnArgs& a, const Dies& d, uint32_t slot, char* lds, Item& it) {
+__device__ __forceinline__ Item find_item(const AttnArgs& a, const Dies& d, uint32_t slot, char* lds) {
   const int tid = threadIdx.x;
+  const Item none{-1, 0, 0, 0, 0, 0, 0, 0, Request{}};
   if constexpr (!PAGED) {
     const Request r = request<PAGED>(a, 0);
     const int tiles = tile_count<PAGED>(a, r);
-    it.r = r;
-    it.length = a.length;
     if (a.length < kUncut) {
       const int parts = (tile_blocks(a, r) + a.length - 1) / a.length, each = a.heads_kv * tiles * parts;
       const uint32_t total = (uint32_t)a.batch * each, x = d.eighth(slot, total);
-      if (x >= total) return false;
+      if (x >= total) return none;
       const int b = x / each;
-      d.part(b, tiles, parts, (int)(x - b * each), b * each, b * a.heads_kv * tiles, it);
+      return d.part(r, b, tiles, parts, a.length, (int)(x - b * each), b * each, b * a.heads_kv * tiles);
     } else {
       // `step` consecutive requests' tiles of a head are dealt to the dies evenly.
       const uint32_t each = (uint32_t)(a.heads_kv / d.h * tiles);
       int b = (int)(slot / each) * d.step, rel = (int)(slot % each);
       while (b < a.batch && rel >= d.items_of(b, tiles)) rel -= d.items_of(b++, tiles);
-      if (b >= a.batch) return false;
-      d.whole(b, tiles, rel, it);
+      return b < a.batch ? d.whole(r, b, tiles, rel) : none;
     }
   } else {
     __shared__ uint32_t wave_sum[TTHREADS / 64][3];
@@ -1368,7 +1357,6 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, const Dies& d, uint
     if (tid == 0) {
       longest = 0;
       found.b = -1;
-      found.length = kUncut;
     }
     __syncthreads();
     // All tiles (at most 256 a request: only fewer in all matter) and this die's
@@ -1437,7 +1425,7 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, const Dies& d, uint
       }
       x = d.eighth(slot, total);
     }
-    if (x >= total) return false;           // uniform
+    if (x >= total) return none;            // uniform
     if (before <= x && x - before < mine) {
       uint32_t rel = x - before;
       for (int b = b0; b < b1; ++b) {
@@ -1452,31 +1440,15 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, const Dies& d, uint
           tiles_before += a.heads_kv * tiles;
           continue;
         }
-        Item mine;
-        if (cut)
-          d.part(b, tiles, parts, (int)rel, (int)before, (int)tiles_before, mine);
-        else
-          d.whole(b, tiles, (int)rel, mine);
-        mine.length = length;
-        mine.r = r;
-        found = mine;
+        found = cut ? d.part(r, b, tiles, parts, length, (int)rel, (int)before, (int)tiles_before)
+                    : d.whole(r, b, tiles, (int)rel);
         break;
       }
     }
     __syncthreads();
-    it = found;
-    if (it.b < 0) return false;             // requests that overlap, counted past 32 bits
+    // None: requests that overlap, counted past 32 bits.
+    return found.b < 0 ? none : found;
   }
-  it.b = uniform(it.b);
-  it.hk = uniform(it.hk);
-  it.tile = uniform(it.tile);
-  it.part = uniform(it.part);
-  it.parts = uniform(it.parts);
-  it.length = uniform(it.length);
-  it.index = uniform(it.index);
-  it.tile_index = uniform(it.tile_index);
-  it.r = uniform(it.r);
-  return true;
 }
 
 // In a mixed launch the workgroups from a.tile_groups on do the row kernel's work, in
@@ -1493,11 +1465,12 @@ fa_serve_tiles_kernel(AttnArgs a) {
       return;
     }
   const Dies d(blockIdx.x & 7, a.heads_kv);
-  Item it;
-  const bool some = find_item<BF, PAGED>(a, d, blockIdx.x >> 3, lds, it);
+  const Item found = find_item<BF, PAGED>(a, d, blockIdx.x >> 3, lds);
+  const Item it{uniform(found.b),      uniform(found.hk),    uniform(found.tile),       uniform(found.part), uniform(found.parts),
+                uniform(found.length), uniform(found.index), uniform(found.tile_index), uniform(found.r)};
   if (!PAGED && blockIdx.x == 0 && threadIdx.x == 0 && a.split)
     a.tdesc[0] = a.length < kUncut ? a.batch * a.heads_kv * tile_count<PAGED>(a, request<PAGED>(a, 0)) : 0;
-  if (!some) return;
+  if (it.b < 0) return;                     // no item
   if (it.length < kUncut && it.part == 0 && threadIdx.x == 0) {
     int* desc = a.tdesc + (it.tile_index + 1) * DESC_INTS;
     desc[0] = it.b;
