@@ -770,20 +770,18 @@ fa_serve_rows_kernel(AttnArgs a) {
 // many pieces an item has. Up to kFewPieces pieces, 32 lanes take a row (4 dims each),
 // 8 rows at once; beyond, the workgroup takes a quarter of a row's dims at a
 // time, 32 groups of 8 lanes reading a 32nd of the pieces each.
-// Both forms have as many loads in flight as there are pieces to a lane: the first
-// form alone took 23.6 us for one row's 512 pieces (131072 keys), a workgroup a row
-// 16.6 us for 8 rows of 2 or 3 (64 requests).
+// Both forms have their loads in flight at once: the first form alone took 23.6 us
+// for the 12 rows' 512 pieces of 131072 keys (the second 6.9), a workgroup a row
+// 16.6 us for 8 rows of 2 or 3 pieces (64 requests).
 constexpr int kFewPieces = 32;
 template <bool BF, bool PAGED>
 __device__ __forceinline__ void merge_rows(const AttnArgs& a, int block) {
-  __shared__ float weight[kRowsGroups];
-  __shared__ float red[32][36];             // padded: 8 rows of 4 lanes' dims at a time
-  __shared__ float wave_red[4];
+  __shared__ float red[32][36];             // 32 dims, the maximum and the sum of a group
   const int* desc = a.desc + (block + 1) * DESC_INTS;
   const int first = desc[3];
   if (first < 0) return;
   const int b = desc[0], hk = desc[1], tile = desc[2], last = desc[4], row0 = desc[5];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x;
   const int boundaries = last - first, pieces = boundaries + 1, mine = block - first;
   const int rows = min(desc[6] - tile * RT, RT);
   auto piece = [&](int s) { return 2 * (first + s) + (s == 0); };
@@ -820,12 +818,15 @@ __device__ __forceinline__ void merge_rows(const AttnArgs& a, int block) {
         if (s0) read(s0);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          if (s0 + e >= pieces) break;      // not by a weight of 0: the last piece may hold an infinity
-          const float ws = __shfl(w, s0 + e, 32);
-          o.x = __builtin_fmaf(ws, v[e].x, o.x);
-          o.y = __builtin_fmaf(ws, v[e].y, o.y);
-          o.z = __builtin_fmaf(ws, v[e].z, o.z);
-          o.w = __builtin_fmaf(ws, v[e].w, o.w);
+          // Past the last piece both factors are 0: that piece, read again, may hold an
+          // infinity. (Leaving the loop there makes the loads wait for each other:
+          // 7.2 us instead of 4.0 for 17 pieces.)
+          const bool on = s0 + e < pieces;
+          const float ws = on ? __shfl(w, min(s0 + e, 31), 32) : 0.f;
+          o.x = __builtin_fmaf(ws, on ? v[e].x : 0.f, o.x);
+          o.y = __builtin_fmaf(ws, on ? v[e].y : 0.f, o.y);
+          o.z = __builtin_fmaf(ws, on ? v[e].z : 0.f, o.z);
+          o.w = __builtin_fmaf(ws, on ? v[e].w : 0.f, o.w);
         }
       }
       const float inv = total == 0.f ? 0.f : 1.f / total;
@@ -837,50 +838,53 @@ __device__ __forceinline__ void merge_rows(const AttnArgs& a, int block) {
   }
   for (int u = mine; u < 4 * rows; u += boundaries) {
     const int n = u >> 2, dim = (u & 3) * 32 + (tid & 7) * 4, grp = tid >> 3;
-    float x[kRowsGroups / 256], M = -INFINITY;
+    // The group's pieces, s = grp, grp + 32, .., joined on their own; all loads at once.
+    constexpr int EACH = kRowsGroups / 32;
+    float4 v[EACH];
+    float x[EACH], M = -INFINITY, total = 0.f;
 #pragma unroll
-    for (int k = 0; k < kRowsGroups / 256; ++k) {
-      const int s = tid + 256 * k;
-      x[k] = s < pieces ? a.lpart[piece(s) * RT + n] : -INFINITY;
+    for (int k = 0; k < EACH; ++k) {
+      const int at = piece(min(grp + 32 * k, boundaries)) * RT + n;
+      x[k] = a.lpart[at];
+      v[k] = *reinterpret_cast<const float4*>(a.opart + (int64_t)at * HD + dim);
+    }
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      x[k] = grp + 32 * k < pieces ? x[k] : -INFINITY;
       M = smax(M, x[k]);
     }
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) M = smax(M, __shfl_xor(M, d));
-    __syncthreads();                        // the last unit's LDS has been read
-    if (lane == 0) wave_red[wave] = M;
-    __syncthreads();
-    M = smax(smax(wave_red[0], wave_red[1]), smax(wave_red[2], wave_red[3]));
-    float total = 0.f;
-#pragma unroll
-    for (int k = 0; k < kRowsGroups / 256; ++k) {
-      const float w = x[k] == -INFINITY ? 0.f : expf(x[k] - M);
-      weight[tid + 256 * k] = w;
-      total += w;
-    }
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) total += __shfl_xor(total, d);
-    __syncthreads();
-    if (lane == 0) wave_red[wave] = total;
     float4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < kRowsGroups / 32; ++k) {
-      const int s = grp + 32 * k;
-      if (s < pieces) {
-        const float4 v = *reinterpret_cast<const float4*>(a.opart + (piece(s) * RT + n) * HD + dim);
-        const float w = weight[s];
-        o.x = __builtin_fmaf(w, v.x, o.x);
-        o.y = __builtin_fmaf(w, v.y, o.y);
-        o.z = __builtin_fmaf(w, v.z, o.z);
-        o.w = __builtin_fmaf(w, v.w, o.w);
-      }
+    for (int k = 0; k < EACH; ++k) {
+      const bool on = x[k] != -INFINITY;    // such a piece, and with a visible key
+      const float w = on ? expf(x[k] - M) : 0.f;
+      total += w;
+      o.x = __builtin_fmaf(w, on ? v[k].x : 0.f, o.x);
+      o.y = __builtin_fmaf(w, on ? v[k].y : 0.f, o.y);
+      o.z = __builtin_fmaf(w, on ? v[k].z : 0.f, o.z);
+      o.w = __builtin_fmaf(w, on ? v[k].w : 0.f, o.w);
     }
+    __syncthreads();                        // the last unit's LDS has been read
     *reinterpret_cast<float4*>(&red[grp][(tid & 7) * 4]) = o;
+    if ((tid & 7) == 0) {
+      red[grp][32] = M;
+      red[grp][33] = total;
+    }
     __syncthreads();
     if (tid < 32) {
-      total = (wave_red[0] + wave_red[1]) + (wave_red[2] + wave_red[3]);
-      float sum = 0.f;
+      M = -INFINITY;
 #pragma unroll
-      for (int s = 0; s < 32; ++s) sum += red[s][tid];
+      for (int s = 0; s < 32; ++s) M = smax(M, red[s][32]);
+      float sum = 0.f;
+      total = 0.f;
+#pragma unroll
+      for (int s = 0; s < 32; ++s) {
+        const float m = red[s][32];
+        if (m == -INFINITY) continue;
+        const float w = expf(m - M);
+        total = __builtin_fmaf(w, red[s][33], total);
+        sum = __builtin_fmaf(w, red[s][tid], sum);
+      }
       const float inv = total == 0.f ? 0.f : 1.f / total;
       reinterpret_cast<uint16_t*>(out_row(n))[(u & 3) * 32 + tid] = narrow<BF>(sum * inv);
       if ((u & 3) == 0 && tid == 0) out_lse(n, M, total);

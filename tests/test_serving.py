@@ -301,3 +301,21 @@ def test_host_sanitizer_build_leaves_device_code_alone():
     sanitizers = [i for i, f in enumerate(flags) if f.startswith("-fsanitize")]
     assert sanitizers and all(flags[i - 1] == "-Xarch_host" for i in sanitizers)
     assert build.SERVING_HOSTSAN not in build.TARGETS and build.SERVING in build.TARGETS
+
+
+def test_measured_work_counts_what_is_visible():
+    from fa_amd.measure import serving as measure
+
+    for window, sinks in ((None, 0), (1, 0), (5, 0), (5, 3), (40, 7)):
+        for past, new in ((0, 1), (0, 9), (13, 4), (50, 20)):
+            rows = [[j for j in range(p + 1) if window is None or j > p - window or j < sinks]
+                    for p in range(past, past + new)]
+            assert measure.visible_pairs(past, new, window, sinks) == sum(map(len, rows))
+            keys = set().union(*rows)
+            step = measure.Step("x", 4, 2, ((past, new), (3, 1)), window, sinks)
+            other = [j for j in range(4) if window is None or j > 3 - window or j < sinks]
+            assert measure.work(step) == (512 * ((new + 1) * 4 + 2 * (len(keys) + len(other))),
+                                          512 * 4 * (sum(map(len, rows)) + len(other)))
+    lines = measure.render([{"name": "x", "plan": 1.0, "store": 2.0, "attend": 3.0, "tbs": 4.0, "tflops": 5.0}],
+                           "float16", "python -m fa_amd.measure.serving")
+    assert lines[1] == "command: python -m fa_amd.measure.serving" and "4.00" in lines[3]
