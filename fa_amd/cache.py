@@ -63,8 +63,8 @@ class PagedCache:
         ints = dict(dtype=torch.int32, device=device)
         self.table = torch.full((config.max_batch, -(-config.max_length // config.page_size)), -1, **ints)
         self.lengths = torch.zeros(config.max_batch, **ints)
-        # Free pages from index `taken` on, and an entry that release() may write to.
-        self.pages = torch.arange(config.pages + 1, **ints)
+        # Free pages from index `taken` on, behind those in use.
+        self.pages = torch.arange(config.pages, **ints)
         self.taken = torch.zeros(1, **ints)
         self.plan = None
         self.max_new = 1
@@ -74,9 +74,10 @@ class PagedCache:
         sits out) and returns the step's ``PagePlan``: positions and slots of
         ``tokens`` rows, request by request (more than the sum of ``new``: the
         rest belongs to none). ``max_new`` bounds the entries of ``new``. When the
-        pages do not suffice, ``taken`` exceeds their number and the rows
-        without a page get NaN."""
-        self.plan = self.planner(self.lengths, new, self.table, self.pages[:-1], self.taken, tokens)
+        pages do not suffice, the plan's ``taken`` exceeds their number and the rows
+        that read a missing one get NaN, as all rows of a request longer than
+        ``max_length`` do, until release()."""
+        self.plan = self.planner(self.lengths, new, self.table, self.pages, self.taken, tokens)
         self.lengths.copy_(self.plan.key_lengths)
         self.taken.copy_(self.plan.taken)
         self.max_new = max_new
@@ -94,17 +95,18 @@ class PagedCache:
                               plan.key_lengths, self.max_new, return_lse=return_lse)
 
     def release(self, request):
-        """Ends a request: its pages are free again and its number too."""
+        """Ends a request: its pages are free again and its number too. The list of
+        pages is made anew from the block tables, so pages that were counted as taken
+        but never entered (see ``begin``) are free again as well."""
         import torch
 
         if not 0 <= request < self.config.max_batch:
             raise ValueError(f"request must be 0 .. {self.config.max_batch - 1}")
-        size = self.config.page_size
-        held = (self.lengths[request] + size - 1).div(size, rounding_mode="floor")
-        column = torch.arange(self.table.shape[1], device=self.table.device)
-        # Back in front of the free ones; columns without a page go to the spare entry.
-        at = torch.where(column < held, self.taken - held + column, self.config.pages)
-        self.pages[at.long()] = self.table[request]
-        self.taken -= held
         self.table[request] = -1
         self.lengths[request] = 0
+        # A flag a page, and one that the empty entries (-1) set.
+        used = torch.zeros(self.config.pages + 1, dtype=torch.int32, device=self.table.device)
+        used[self.table.flatten().long()] = 1
+        used = used[:-1]
+        self.pages.copy_(torch.sort(used, descending=True, stable=True).indices)
+        self.taken.copy_(used.sum())

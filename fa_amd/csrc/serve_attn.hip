@@ -29,7 +29,8 @@
 // A key that the mask hides has its score replaced by -inf, so NaN in its K has
 // no effect; NaN or an infinity in its V would get into O through the product
 // 0 * NaN in the blocks that take the mask. That is found at the end (l is a
-// number and O is not) and the row computed again key by key (repair_row).
+// number and O is not) and the row computed again key by key, if no visible key
+// accounts for the NaN (spoiled_row, repair_row).
 
 #include <math.h>
 
@@ -97,10 +98,6 @@ __device__ __forceinline__ ConstArgs& fresh_args() {
 // one, are made in vector registers).
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ uint64_t uniform(uint64_t x) {
-  return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) |
-         (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
-}
 
 // Sum over this lane and the lanes before it.
 __device__ __forceinline__ uint32_t lanes_sum(uint32_t x) {
@@ -218,7 +215,7 @@ __device__ __forceinline__ uint32_t low_bits(int n) {
 // Replaces the scores of the keys a row does not see by -inf: those past hi, and those
 // that are neither from lo on nor before sink, all relative to the lane's first key
 // (register r of 32-key tile t holds key 32t + 8 (r / 4) + r % 4 from there). The
-// keys of a tile become a word of hidden bits, of which each score takes one:
+// keys of a tile become a word with a bit for each key seen, of which a score takes its own:
 // two instructions a score. Compares and selects would keep a scalar register
 // pair a score alive; sign arithmetic with its three differences a score made a
 // block with the mask take 2.3 us longer than one without.
@@ -235,7 +232,7 @@ __device__ __forceinline__ void hide(f32x16 (&s)[T], int hi, int lo, int sink) {
   }
 }
 
-// One step of the online softmax over N scores of the lane's row (the other
+// One step of the online softmax over 16 T scores of the lane's row (the other
 // half of the keys is with lane + 32): raises m, rescales l and O if some row of
 // the wave needs it, and turns the scores into P fragments. at(i) runs before
 // the exponentials of pair i.
@@ -350,10 +347,59 @@ struct Stream {
   }
 };
 
+// Exponent all ones: infinity or NaN, in the lower (1) and the upper (2) element of a word.
+template <bool BF>
+__device__ __forceinline__ int not_finite(uint32_t w) {
+  constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
+  return ((w & E) == E ? 1 : 0) | ((w >> 16 & E) == E ? 2 : 0);
+}
+
+// Whether a row whose O has NaN in it must be computed again: some dim has infinity or
+// NaN in the V of a key that the row does not see (in the blocks [s0, s1) of a list, which
+// it was computed from), and the keys that it sees hold neither NaN nor infinities of both
+// signs there, which would be the row's own NaN. The whole wave works on one row, 2 dims
+// a lane. Both passes end early: a V that is NaN all over costs a row a few keys.
+template <bool BF, bool PAGED, typename Args, typename BlockAt>
+__device__ __forceinline__ bool spoiled_row(const Args& a, const Stream<PAGED>& st, int pos, int s0, int s1,
+                                            BlockAt&& block_at) {
+  constexpr int STEP = 4;                   // keys whose loads are in flight together
+  const int lane = threadIdx.x & 63;
+  const int hi = min(pos, st.keys - 1);
+  int hidden = 0;                           // dims (a bit each) not finite at a hidden key
+  float seen[2] = {0.f, 0.f};               // the sum of what is not finite at visible ones
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int s = s0; s < s1; ++s) {
+      const int key0 = block_at(s) * BLOCK;
+      if (pass == 0 && key0 + BLOCK - 1 <= hi && (key0 > pos - a.window || key0 + BLOCK <= a.sinks)) continue;
+      for (int key = key0; key < key0 + BLOCK && key < st.keys; key += STEP) {
+        uint32_t w[STEP];
+#pragma unroll
+        for (int e = 0; e < STEP; ++e)
+          w[e] = *reinterpret_cast<const uint32_t*>(st.v + st.at(min(key + e, st.keys - 1), a.vs_b, a.vs_n) + 4 * lane);
+#pragma unroll
+        for (int e = 0; e < STEP; ++e) {
+          if (key + e >= st.keys) continue;
+          const bool visible = key + e <= hi && (key + e > pos - a.window || key + e < a.sinks);
+          const int odd = not_finite<BF>(w[e]);
+          if (!visible) {
+            hidden |= odd;
+          } else if (pass) {
+            seen[0] += odd & 1 ? widen<BF>((uint16_t)w[e]) : 0.f;
+            seen[1] += odd & 2 ? widen<BF>((uint16_t)(w[e] >> 16)) : 0.f;
+          }
+        }
+        const int left = hidden & ((seen[0] == seen[0] ? 1 : 0) | (seen[1] == seen[1] ? 2 : 0));
+        if (pass && !__builtin_amdgcn_ballot_w64(left != 0)) return false;
+      }
+    }
+    if (!pass && !__builtin_amdgcn_ballot_w64(hidden != 0)) return false;
+  }
+  return true;
+}
+
 // A row again, one key at a time, over the blocks [s0, s1) of a list: o (dims
-// 2 lane, 2 lane + 1) and lse of the keys it sees, which alone are read. The
-// whole wave works on one row; for the rare rows that NaN in a hidden key's V
-// has reached.
+// 2 lane, 2 lane + 1) and lse of the keys it sees, which alone are read; for the rare
+// rows that spoiled_row finds.
 template <bool BF, bool PAGED, typename Args, typename BlockAt>
 __device__ __forceinline__ void repair_row(const Args& a, const Stream<PAGED>& st, const char* qrow, int pos,
                                            int s0, int s1, BlockAt&& block_at, float (&o)[2], float& lse) {
@@ -611,9 +657,10 @@ __device__ __forceinline__ void row_item(const AttnArgs& a, const Request& r, in
   while (sick) {
     const int at = __ffsll((unsigned long long)sick) - 1;
     sick &= ~(0xffull << (at & ~7));
-    again |= (lane >> 3) == (at >> 3);
     const int row = tile * RT + __builtin_amdgcn_readfirstlane(__shfl(n, at));
     const int ri = row / a.group, rh = hk * a.group + row % a.group;
+    if (!spoiled_row<BF, PAGED>(a, st, r.pos + ri, s0, s1, block_at)) continue;
+    again |= (lane >> 3) == (at >> 3);
     float x[2], rl;
     repair_row<BF, PAGED>(a, st, a.q + b * a.qs_b + (int64_t)(r.row0 + ri) * a.qs_n + rh * a.qs_h, r.pos + ri, s0, s1,
                           block_at, x, rl);
@@ -1222,11 +1269,13 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
   uint64_t again = __builtin_amdgcn_ballot_w64(sick);
   again |= again >> 32;
   again &= 0xffffffffull;                   // a bit a row
-  const uint32_t repaired = (uint32_t)again;
+  uint32_t repaired = 0;
   while (again) {
     const int n = __ffsll((unsigned long long)again) - 1;
     again &= again - 1;
     const int rr = row0 + n, ri = rr / f.group, rh = hk * f.group + rr % f.group;
+    if (!spoiled_row<BF, PAGED>(f, st, r.pos + ri, 0, nblk, block_at)) continue;
+    repaired |= 1u << n;
     float x[2], rl;
     repair_row<BF, PAGED>(f, st, f.q + b * f.qs_b + (int64_t)(r.row0 + ri) * f.qs_n + rh * f.qs_h, r.pos + ri, 0, nblk,
                           block_at, x, rl);
@@ -1634,6 +1683,14 @@ int check_type(int32_t type) {
 // Rows of K and V within a page (or of a contiguous tensor) are 32-bit apart.
 int check_rows(int64_t stride) { return stride < HD || stride >= 1 << 25 ? FA_SERVE_ERR_STRIDE : FA_SERVE_OK; }
 
+// A workgroup for every item there can be: each die's share of whole tiles rounds
+// up once a request and head.
+int64_t tile_groups(const LaunchPlan& lp, int64_t batch, int64_t heads_kv) {
+  const int64_t h = std::min<int64_t>(heads_kv & -heads_kv, 8);
+  const int64_t grid = 8 * (lp.tiles_max / 8 + heads_kv / h * batch + 1);
+  return std::max<int64_t>(grid, lp.split ? kTileItems : 8);
+}
+
 int run(const AttnArgs& filled, const LaunchPlan& lp, int32_t type, bool paged, void* workspace, void* stream) {
   AttnArgs a = filled;
   int rc = check_stream_device(stream);
@@ -1653,11 +1710,7 @@ int run(const AttnArgs& filled, const LaunchPlan& lp, int32_t type, bool paged, 
   const Kernels& k = kKernels[type == FA_SERVE_BF16][paged];
   void* args[] = {&a};
   if (lp.tiles) {
-    // A workgroup for every item there can be: each die's share of whole tiles
-    // rounds up once a request and head.
-    const int64_t h = std::min<int64_t>(a.heads_kv & -(int64_t)a.heads_kv, 8);
-    const int64_t grid = 8 * (lp.tiles_max / 8 + a.heads_kv / h * a.batch + 1);
-    a.tile_groups = (int)std::max<int64_t>(grid, lp.split ? kTileItems : 8);
+    a.tile_groups = (int)tile_groups(lp, a.batch, a.heads_kv);
     rc = enqueue(lp.rows ? k.mixed : k.tiles, dim3((unsigned)(a.tile_groups + a.groups)), dim3(TTHREADS), args,
                  kTileLds, stream);
   } else {
@@ -1670,9 +1723,10 @@ int run(const AttnArgs& filled, const LaunchPlan& lp, int32_t type, bool paged, 
 }
 
 // The row kernel counts the key blocks of all its items in 32 bits; the tile
-// kernel's launch has a workgroup a tile.
+// kernel's launch has fewer than 2^32 threads.
 int check_work(const LaunchPlan& lp, int64_t batch, int64_t heads_kv, int64_t group, int64_t rows, int64_t keys) {
-  if (lp.tiles && lp.tiles_max + heads_kv * batch >= 1 << 22) return FA_SERVE_ERR_GEOMETRY;
+  if (lp.tiles && tile_groups(lp, batch, heads_kv) + kRowsGroups >= ((int64_t)1 << 32) / TTHREADS)
+    return FA_SERVE_ERR_GEOMETRY;
   if (!lp.rows) return FA_SERVE_OK;
   const int64_t tiles = lp.tiles ? batch * (kRowsMax / RT) : rows * group / RT + batch;
   return tiles <= ((int64_t)1 << 31) / heads_kv / (keys / BLOCK + 2) ? FA_SERVE_OK : FA_SERVE_ERR_GEOMETRY;

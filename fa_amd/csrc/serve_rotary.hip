@@ -134,7 +134,8 @@ int fa_rotary_append(const fa_rotary* p, const void* q, void* q_out, const void*
                      void* k_cache, void* v_cache, void* stream) {
   if (!p) return FA_SERVE_ERR_NULL;
   const int64_t limit = (int64_t)1 << 30;
-  if (p->tokens < 0 || p->tokens > limit || p->heads_q < 0 || p->heads_kv < 0 || p->heads_q > 4096 ||
+  // 8 threads a token, and fewer than 2^32 threads in a dimension of a launch.
+  if (p->tokens < 0 || p->tokens > limit / 4 || p->heads_q < 0 || p->heads_kv < 0 || p->heads_q > 4096 ||
       p->heads_kv > 4096 || p->heads_q + p->heads_kv < 1)
     return FA_SERVE_ERR_GEOMETRY;
   if (p->type != FA_SERVE_FP16 && p->type != FA_SERVE_BF16) return FA_SERVE_ERR_TYPE;

@@ -22,6 +22,7 @@ call waits for the GPU or copies from it. The reference has no counterpart.
 
 import ctypes as C
 import math
+import numbers
 from collections import namedtuple
 from dataclasses import dataclass
 
@@ -178,6 +179,7 @@ class _Operator:
 
 
 ALIGN_ERROR = f"rows of {DIM} dims must be 16-byte aligned"
+OUT_ERROR = "out must not be a tensor that the call reads"
 
 
 class PagePlanner(_Operator):
@@ -317,7 +319,8 @@ class Rotary(_Operator):
 
     ``rotary(x, positions)`` rotates x [T, H, 128] (any strides of T and H) at
     ``positions`` [T]; with ``backward=True`` it is the rotation's transpose,
-    which takes a gradient of the rotated tensor to one of x. ``out`` may be x.
+    which takes a gradient of the rotated tensor to one of x. ``out`` may be x
+    (with its strides), and overlaps x in no other way.
 
     ``rotary.append(q, k, v, positions, slots, k_cache, v_cache)`` returns q
     rotated and stores k, rotated, and v at ``slots`` [T] of the caches
@@ -441,6 +444,8 @@ def _check_mask(window, sinks):
 
 
 def _check_scale(scale):
+    if scale is not None and not isinstance(scale, numbers.Real):
+        raise ValueError("scale must be a number")
     scale = DIM ** -0.5 if scale is None else float(scale)
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError("scale must be finite and positive")
@@ -474,7 +479,8 @@ class PagedAttention(_Operator):
 
     Returns o [T, heads_q, 128], with ``return_lse`` also the rows'
     log-sum-exp [T, heads_q] FP32. Rows behind the last request are left as
-    they were in ``out`` (undefined without ``out``). A row that sees no key
+    they were in ``out`` (undefined without ``out``; ``out`` must not overlap what
+    the call reads). A row that sees no key
     gets 0 and -inf. A request that is longer than its table row, or whose table
     names a page that the cache does not have, gets NaN where that is read."""
 
@@ -507,6 +513,8 @@ class PagedAttention(_Operator):
         qp, kc, vc, op = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
         if (qp | kc | vc | op) % 16:
             raise ValueError(ALIGN_ERROR)
+        if op and op in (qp, kc, vc):
+            raise ValueError(OUT_ERROR)
         self.launch(self.lib.fa_paged_fwd,
                     (prob, qp, kc, vc, table.data_ptr(), query_starts.data_ptr(),
                      key_lengths.data_ptr(), op, lse.data_ptr() if return_lse else None,
@@ -581,7 +589,7 @@ class WindowAttention(_Operator):
     """Callable ``(q, k, v) -> o`` (``fa_window_fwd``): q [B, Hq, Nq, 128], k and v
     [B, Hkv, Nk, 128], any strides of the first three dims; with ``return_lse``
     also the rows' log-sum-exp [B, Hq, Nq] FP32. A row that sees no key gets 0
-    and -inf."""
+    and -inf. ``out`` must not overlap what the call reads."""
 
     def __init__(self, config, library=None):
         super().__init__(library)
@@ -604,6 +612,8 @@ class WindowAttention(_Operator):
         qp, kp, vp, op = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
         if (qp | kp | vp | op) % 16:
             raise ValueError(ALIGN_ERROR)
+        if op in (qp, kp, vp):
+            raise ValueError(OUT_ERROR)
         self.launch(self.lib.fa_window_fwd,
                     (prob, qp, kp, vp, op, lse.data_ptr() if return_lse else None, ws.data_ptr(),
                      size), device, (q, k, v, out))

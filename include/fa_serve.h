@@ -99,7 +99,7 @@ int fa_plan_pages(const fa_page_plan* p, const int32_t* past, const int32_t* fre
  * rotated to k_cache, v unrotated to v_cache, at slots[t]; a token whose slot
  * is negative or past the cache is not stored. Slots of one call that are
  * stored are distinct. heads_kv = 0 leaves out k, v, the caches and slots.
- * q_out may be q.
+ * q_out may be q, with q's strides; no other two tensors overlap.
  */
 enum fa_rotary_layout { FA_ROTARY_HALF = 0, FA_ROTARY_INTERLEAVED = 1 };
 typedef struct fa_rotary {
@@ -134,6 +134,8 @@ int fa_rotary_append(const fa_rotary* p, const void* q, void* q_out, const void*
  * outside 0 .. tokens are clamped. A row gets NaN if its request is longer than
  * its table row (max_pages * page_size) or a page its tile reads is outside
  * 0 .. pages-1.
+ *
+ * o overlaps nothing that the call reads: rows are written while others are read.
  *
  * Workspace: fa_paged_workspace_bytes(); its contents on entry do not matter.
  * Calls that may overlap need a workspace each.

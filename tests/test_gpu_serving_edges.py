@@ -70,6 +70,33 @@ def check_values(batch, o, lse, window=None, sinks=0):
 
 
 @pytest.mark.parametrize("spans,heads,page", HIDDEN)
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_infinities_beside_a_hidden_nan(lib, spans, heads, page, dtype):
+    # A dim with NaN at the newest key and infinities at older ones: rows before it
+    # keep the infinity of what they see, and NaN where they see both signs.
+    inf = float("inf")
+    batch = Batch(spans, heads, page, dtype, seed=9)
+    past, new = spans[0]
+    last, first = past + new - 1, min(5, past + new - 2)
+    at = lambda key: (batch.table[0][key // page], key % page)
+    batch.v[at(last)] = float("nan")
+    batch.v[at(first)][..., 0:2] = inf
+    batch.v[at(first)][..., 8] = inf
+    batch.v[at(first + 1)][..., 8] = -inf
+    batch.v[at(first + 1)][..., 9] = -inf
+    o, lse = run(batch, lib)
+    check_values(batch, o, lse)
+
+
+@pytest.mark.parametrize("spans,heads,page", HIDDEN + [([(30000, 200), (30000, 2)], (8, 1), 32)])
+def test_values_of_nan_alone(lib, spans, heads, page):
+    batch = Batch(spans, heads, page, "fp16", seed=10)
+    batch.v[:] = float("nan")
+    o, lse = run(batch, lib)
+    check_values(batch, o, lse)
+
+
+@pytest.mark.parametrize("spans,heads,page", HIDDEN)
 @pytest.mark.parametrize("window,sinks", [(40, 0), (40, 3)])
 def test_nan_outside_the_window(lib, spans, heads, page, window, sinks):
     batch = Batch(spans, heads, page, "fp16", seed=8)
@@ -114,6 +141,19 @@ def test_scores_far_below_zero(lib, new):
         tol = 2.01 * 2.0 ** -8 * want.abs() + 2.0 ** -18 * v.abs().mean(0)
         compare(o[i, 0].cpu(), want, tol)
     assert torch.isfinite(lse).all() and (lse < -1e6).all()
+
+
+@pytest.mark.parametrize("spans,heads", [([(100000, 1)], (12, 1)), ([(100000, 1)] * 3, (4, 2)),
+                                         ([(20000, 130)], (2, 1))])
+def test_a_nan_score_in_one_of_many_pieces(lib, spans, heads):
+    # The joins: a piece whose log-sum-exp is NaN among hundreds of others.
+    batch = Batch(spans, heads, 64, "bf16", seed=11)
+    at = spans[0][0] * 3 // 4
+    batch.k[batch.table[0][at // 64], at % 64, 0] = float("nan")
+    o, lse = run(batch, lib)
+    check_values(batch, o, lse)
+    own = slice(0, spans[0][1]), slice(0, heads[0] // heads[1])
+    assert o[own].isnan().all() and lse[own].isnan().all()
 
 
 # Lengths, tables, padding.
@@ -477,3 +517,35 @@ def test_a_cache_over_several_steps(lib, window, sinks, dtype, page):
                 for h in range(4):
                     x = attend64(qr[rows, h], ks[:, h // 2], vs[:, h // 2], pos, key, window, sinks, 128 ** -0.5)
                     compare(o[rows, h].cpu(), x[0], bounds(kind, *x, lengths[b])[0])
+
+
+def test_out_must_not_be_what_is_read(lib):
+    batch = Batch([(40, 3)], (2, 2), 16, "fp16")
+    args = batch.gpu()
+    with pytest.raises(ValueError, match="out"):
+        PagedAttention(library=lib)(*args, out=args[0])
+    q = torch.zeros(1, 2, 40, 128, dtype=torch.float16, device="cuda")
+    for t in ([q, torch.zeros_like(q), torch.zeros_like(q)], [torch.zeros_like(q), q, torch.zeros_like(q)]):
+        with pytest.raises(ValueError, match="out"):
+            WindowAttention(WindowConfig(window=8), library=lib)(*t, out=q)
+
+
+def test_a_cache_that_was_asked_for_too_much(lib):
+    # 11 pages of 16 tokens for 20, 100 and 60 tokens: the last request misses two
+    # pages and gets NaN; once it has ended, the others go on and its pages serve a new one.
+    cache = PagedCache(CacheConfig(layers=1, heads_q=2, heads_kv=1, pages=11, page_size=16, max_batch=3,
+                                   max_length=160))
+    torch.manual_seed(6)
+
+    def step(new):
+        tokens = sum(new)
+        q, k, v = (torch.randn(tokens, h, 128).half().cuda() for h in (2, 1, 1))
+        cache.begin(torch.tensor(new, dtype=torch.int32).cuda(), tokens, max(new))
+        return cache.attend(0, q, k, v)
+
+    o = step([20, 100, 60])
+    assert torch.isfinite(o[:120]).all() and o[-12:].isnan().all()
+    cache.release(2)
+    assert sorted(cache.pages.tolist()[int(cache.taken):]) == sorted(set(range(11)) - {
+        i for row in cache.table.tolist() for i in row if i >= 0})
+    assert torch.isfinite(step([1, 1, 30])).all()

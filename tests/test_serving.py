@@ -319,3 +319,58 @@ def test_measured_work_counts_what_is_visible():
     lines = measure.render([{"name": "x", "plan": 1.0, "store": 2.0, "attend": 3.0, "tbs": 4.0, "tflops": 5.0}],
                            "float16", "python -m fa_amd.measure.serving")
     assert lines[1] == "command: python -m fa_amd.measure.serving" and "4.00" in lines[3]
+
+
+def test_refusals_of_launches_past_32_bits(lib):
+    # Threads of a launch: 8 a token (rotary), 512 a tile and die (attention).
+    assert rotary_call(lib, tokens=(1 << 28) + 1) == 2
+    many = dict(batch=4096, heads_q=1023, heads_kv=1023, tokens=4096 * 100)
+    assert paged_call(lib, **many, max_new=100, qs=(1024 * 128, 128)) == 2
+    assert window_call(lib, batch=65535, heads_q=1023, heads_kv=1023, seq_q=100) == 2
+
+
+@pytest.mark.parametrize("scale", [torch.tensor(0.1), "0.1", [0.1]])
+def test_scale_must_be_a_number(scale):
+    # A tensor would be kept by its identity, and read once.
+    with pytest.raises(ValueError, match="number"):
+        serving._check_scale(scale)
+
+
+def small_cache(**kw):
+    from fa_amd.cache import CacheConfig, PagedCache
+
+    config = dict(layers=1, heads_q=1, heads_kv=1, pages=10, page_size=16, max_batch=3, max_length=96)
+    return PagedCache(CacheConfig(**{**config, **kw}), device="cpu")
+
+
+def fill(cache, new):
+    """What begin() leaves in the cache's state, without the GPU."""
+    plan = serving_reference.plan(cache.lengths.tolist(), new, cache.table.tolist(), cache.pages.tolist(),
+                                  int(cache.taken), sum(new), cache.config.page_size)
+    for name, values in (("table", plan[0]), ("lengths", plan[2]), ("taken", [plan[5]])):
+        getattr(cache, name).copy_(torch.tensor(values, dtype=torch.int32))
+
+
+def free_pages(cache):
+    return sorted(cache.pages.tolist()[int(cache.taken):])
+
+
+@pytest.mark.parametrize("steps,end", [
+    ([[40, 20, 90]], 2),                      # 3 + 2 + 6 pages of 10: one is missing
+    ([[90, 0, 0], [0, 50, 90]], 0),           # the missing ones belong to others
+    ([[200, 16, 0]], 0),                      # longer than its table row
+    ([[16, 200, 0], [16, 0, 16]], 1),
+])
+def test_release_after_too_much_was_asked(steps, end):
+    cache = small_cache()
+    for new in steps:
+        fill(cache, new)
+    cache.release(end)
+    held = [i for row in cache.table.tolist() for i in row if i >= 0]
+    assert cache.table[end].eq(-1).all() and int(cache.lengths[end]) == 0
+    assert len(set(held)) == len(held)
+    # Every page that no table names is free, once.
+    assert free_pages(cache) == sorted(set(range(10)) - set(held))
+    for request in range(3):
+        cache.release(request)
+    assert free_pages(cache) == list(range(10))
