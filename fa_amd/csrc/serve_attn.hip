@@ -1595,8 +1595,22 @@ __global__ void __launch_bounds__(256) fa_serve_mixed_merge_kernel(AttnArgs a) {
 // ---------------------------------------------------------------------------
 // Host side.
 
-// A request's packed rows up to this many go to the row kernel.
-constexpr int64_t kRowsMax = 64;
+// Which kernel takes a request (row kernel against tile kernel, FP16, 8 query heads a
+// KV head, 64 heads where not said):
+//   - One row tile: the row kernel. 32 rows of 32 requests of 1000-8000 keys 135 us
+//     against 163, of one request of 8000 keys 21 against 37, of 64 requests of
+//     4000 keys with one KV head 32 against 53.
+//   - More than kRowsMax rows: the tile kernel, as the row kernel reads the keys once a
+//     row tile. 96 rows of 32 requests 288 against 172, of one request 28 against 40, but
+//     of 4 requests of 60000 keys with one KV head 84 against 69.
+//   - In between: the row kernel if the launch has few row tiles. 64 rows of
+//     one request (16 tiles) 26 against 38, of 8 requests of 4000 keys (128) 52 against 47,
+//     of 64 with one KV head (128) 52 against 55, of the 32 (512) 226 against 171; also
+//     beside longer requests, where it fills CUs that have no tile: 20 requests of 48
+//     rows (12 heads, one KV head) and two chunks of 1000 tokens 129 against 149, 10 of
+//     64 rows and two of 2000 tokens 387 against 490; but 58 of 40 rows (8 KV heads)
+//     and two of 300 tokens 261 against 196.
+constexpr int64_t kRowsMax = 64, kRowsItems = 128;
 
 struct Kernels {
   const void *rows, *tiles, *mixed, *rows_merge, *tiles_merge, *mixed_merge;
@@ -1642,8 +1656,10 @@ struct LaunchPlan {
 };
 LaunchPlan launch_plan(int64_t batch, int64_t heads_kv, int64_t group, int64_t tokens, int64_t max_new, bool even) {
   LaunchPlan p;
-  p.rows_max = (int)kRowsMax;
-  p.tiles = max_new * group > kRowsMax;
+  const int64_t most = max_new * group;     // rows of a request
+  const int64_t items = heads_kv * std::min(batch * (kRowsMax / RT), tokens * group / RT + batch);
+  p.tiles = most > (items > kRowsItems ? RT : kRowsMax);
+  p.rows_max = (int)(most > kRowsMax ? kRowsMax : RT);
   // One kernel takes every request if all have few rows, or all as many, or
   // there is one request.
   p.rows = !p.tiles || (batch > 1 && !even);
