@@ -815,15 +815,23 @@ fa_serve_rows_kernel(AttnArgs a) {
 // Workgroup g > 0 whose share starts inside an item is one of the K = pieces - 1 that
 // do, and they share its join, so that a launch's joins are spread evenly however
 // many pieces an item has. Up to kFewPieces pieces, 32 lanes take a row (4 dims each),
-// 8 rows at once; beyond, the workgroup takes a quarter of a row's dims at a
-// time, 32 groups of 8 lanes reading a 32nd of the pieces each.
-// Both forms have their loads in flight at once: the first form alone took 23.6 us
-// for the 12 rows' 512 pieces of 131072 keys (the second 6.9), a workgroup a row
-// 16.6 us for 8 rows of 2 or 3 pieces (64 requests).
-constexpr int kFewPieces = 32;
+// 8 rows at once; up to kSomePieces the workgroup takes a row, 8 groups of 32 lanes
+// reading an 8th of the pieces each; beyond, a quarter of a row, 32 groups of 8 lanes.
+// So every workgroup has one row or quarter to join at most, and all its loads are in
+// flight at once: 34 pieces of 12 rows MIDDLE us, in quarters (which are 48 then) 10; 512
+// pieces of 12 rows in quarters 6.9, as the few are 23.6; 17 pieces as the few 4, in
+// quarters 16.
+constexpr int kFewPieces = 32, MERGE_EACH = 16, kSomePieces = 8 * MERGE_EACH;
+static_assert(32 * MERGE_EACH >= kRowsGroups, "every piece has a load");
+// e^(x - M), 0 for a part that saw no key (also where M is -inf). The product with log2 e
+// is off by half a step of |x - M| log2 e, which the weight it goes with makes
+// smaller than 2^-24.
+__device__ __forceinline__ float weight(float x, float M) {
+  return x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((x - M) * (float)LOG2E);
+}
 template <bool BF, bool PAGED>
 __device__ __forceinline__ void merge_rows(const AttnArgs& a, int block) {
-  __shared__ float red[32][36];             // 32 dims, the maximum and the sum of a group
+  __shared__ __attribute__((aligned(16))) float red[32 * 36];   // results of 32 (or 8) groups
   const int* desc = a.desc + (block + 1) * DESC_INTS;
   const int first = desc[3];
   if (first < 0) return;
@@ -856,7 +864,7 @@ __device__ __forceinline__ void merge_rows(const AttnArgs& a, int block) {
       float M = x;
 #pragma unroll
       for (int d = 16; d >= 1; d >>= 1) M = smax(M, __shfl_xor(M, d, 32));
-      const float w = x == -INFINITY ? 0.f : expf(x - M);
+      const float w = weight(x, M);
       float total = w;
 #pragma unroll
       for (int d = 16; d >= 1; d >>= 1) total += __shfl_xor(total, d, 32);
@@ -883,60 +891,68 @@ __device__ __forceinline__ void merge_rows(const AttnArgs& a, int block) {
     }
     return;
   }
-  for (int u = mine; u < 4 * rows; u += boundaries) {
-    const int n = u >> 2, dim = (u & 3) * 32 + (tid & 7) * 4, grp = tid >> 3;
-    // The group's pieces, s = grp, grp + 32, .., joined on their own; all loads at once.
-    constexpr int EACH = kRowsGroups / 32;
-    float4 v[EACH];
-    float x[EACH], M = -INFINITY, total = 0.f;
+  auto many = [&](auto lanes) {
+    constexpr int LANES = decltype(lanes)::value, GROUPS = 256 / LANES, SLICES = 32 / LANES;
+    constexpr int PITCH = 4 * LANES + 4;    // the dims, the maximum and the sum of a group
+    for (int u = mine; u < SLICES * rows; u += boundaries) {
+      const int n = u / SLICES, dim0 = u % SLICES * 4 * LANES, grp = tid / LANES, l = tid % LANES;
+      // The group's pieces, s = grp, grp + GROUPS, .., joined on their own; all loads at once.
+      float4 v[MERGE_EACH];
+      float x[MERGE_EACH], M = -INFINITY, total = 0.f;
 #pragma unroll
-    for (int k = 0; k < EACH; ++k) {
-      const int at = piece(min(grp + 32 * k, boundaries)) * RT + n;
-      x[k] = a.lpart[at];
-      v[k] = *reinterpret_cast<const float4*>(a.opart + (int64_t)at * HD + dim);
-    }
-#pragma unroll
-    for (int k = 0; k < EACH; ++k) {
-      x[k] = grp + 32 * k < pieces ? x[k] : -INFINITY;
-      M = smax(M, x[k]);
-    }
-    float4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int k = 0; k < EACH; ++k) {
-      const bool on = x[k] != -INFINITY;    // such a piece, and with a visible key
-      const float w = on ? expf(x[k] - M) : 0.f;
-      total += w;
-      o.x = __builtin_fmaf(w, on ? v[k].x : 0.f, o.x);
-      o.y = __builtin_fmaf(w, on ? v[k].y : 0.f, o.y);
-      o.z = __builtin_fmaf(w, on ? v[k].z : 0.f, o.z);
-      o.w = __builtin_fmaf(w, on ? v[k].w : 0.f, o.w);
-    }
-    __syncthreads();                        // the last unit's LDS has been read
-    *reinterpret_cast<float4*>(&red[grp][(tid & 7) * 4]) = o;
-    if ((tid & 7) == 0) {
-      red[grp][32] = M;
-      red[grp][33] = total;
-    }
-    __syncthreads();
-    if (tid < 32) {
-      M = -INFINITY;
-#pragma unroll
-      for (int s = 0; s < 32; ++s) M = smax(M, red[s][32]);
-      float sum = 0.f;
-      total = 0.f;
-#pragma unroll
-      for (int s = 0; s < 32; ++s) {
-        const float m = red[s][32];
-        if (m == -INFINITY) continue;
-        const float w = expf(m - M);
-        total = __builtin_fmaf(w, red[s][33], total);
-        sum = __builtin_fmaf(w, red[s][tid], sum);
+      for (int k = 0; k < MERGE_EACH; ++k) {
+        const int at = piece(min(grp + GROUPS * k, boundaries)) * RT + n;
+        x[k] = a.lpart[at];
+        v[k] = *reinterpret_cast<const float4*>(a.opart + (int64_t)at * HD + dim0 + 4 * l);
       }
-      const float inv = total == 0.f ? 0.f : 1.f / total;
-      reinterpret_cast<uint16_t*>(out_row(n))[(u & 3) * 32 + tid] = narrow<BF>(sum * inv);
-      if ((u & 3) == 0 && tid == 0) out_lse(n, M, total);
+#pragma unroll
+      for (int k = 0; k < MERGE_EACH; ++k) {
+        x[k] = grp + GROUPS * k < pieces ? x[k] : -INFINITY;
+        M = smax(M, x[k]);
+      }
+      float4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < MERGE_EACH; ++k) {
+        const bool on = x[k] != -INFINITY;  // such a piece, and with a visible key
+        const float w = weight(x[k], M);
+        total += w;
+        o.x = __builtin_fmaf(w, on ? v[k].x : 0.f, o.x);
+        o.y = __builtin_fmaf(w, on ? v[k].y : 0.f, o.y);
+        o.z = __builtin_fmaf(w, on ? v[k].z : 0.f, o.z);
+        o.w = __builtin_fmaf(w, on ? v[k].w : 0.f, o.w);
+      }
+      __syncthreads();                      // the last unit's LDS has been read
+      float* const own = red + grp * PITCH;
+      *reinterpret_cast<float4*>(own + 4 * l) = o;
+      if (l == 0) {
+        own[4 * LANES] = M;
+        own[4 * LANES + 1] = total;
+      }
+      __syncthreads();
+      if (tid < 4 * LANES) {
+        M = -INFINITY;
+#pragma unroll
+        for (int s = 0; s < GROUPS; ++s) M = smax(M, red[s * PITCH + 4 * LANES]);
+        float sum = 0.f;
+        total = 0.f;
+#pragma unroll
+        for (int s = 0; s < GROUPS; ++s) {
+          const float* const other = red + s * PITCH;
+          const float m = other[4 * LANES];
+          const float w = weight(m, M);
+          total = __builtin_fmaf(w, other[4 * LANES + 1], total);
+          sum = __builtin_fmaf(w, other[tid], sum);
+        }
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        reinterpret_cast<uint16_t*>(out_row(n))[dim0 + tid] = narrow<BF>(sum * inv);
+        if (dim0 == 0 && tid == 0) out_lse(n, M, total);
+      }
     }
-  }
+  };
+  if (pieces <= kSomePieces)
+    many(std::integral_constant<int, 32>());
+  else
+    many(std::integral_constant<int, 8>());
 }
 
 // ---------------------------------------------------------------------------
@@ -1558,7 +1574,7 @@ __device__ __forceinline__ void merge_tiles(const AttnArgs& a, int block) {
     const float x = a.tlpart[at + (int64_t)s * TT];
     const float4 v = *reinterpret_cast<const float4*>(a.topart + (at + (int64_t)s * TT) * HD + dim);
     if (x == -INFINITY) continue;           // such a part has written no O
-    const float w = expf(x - M);
+    const float w = weight(x, M);
     total += w;
     o.x = __builtin_fmaf(w, v.x, o.x);
     o.y = __builtin_fmaf(w, v.y, o.y);
