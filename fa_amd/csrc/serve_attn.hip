@@ -454,12 +454,16 @@ __device__ __forceinline__ bool is_nan(float x) { return !(x == x); }
 // whatever the requests' lengths; a share starts and ends anywhere in an item. A
 // piece of an item leaves its normalised O and lse in the workspace (a
 // workgroup has at most two, its first and its last), and the merge kernel joins
-// an item's pieces.
+// an item's pieces. Measured, with the joins: 64 requests of 100-8005 keys, 64 heads on 8
+// (470 MB of K and V), 112 us, 4.2 TB/s; 131072 keys of one KV head (67 MB) 22 us, of
+// which the start takes 4 and the join 5; one request of 4099 keys 13 us, all latency.
 constexpr int RT = 32;
 constexpr int RSLOT = 32 * ROW_BYTES;       // 32 keys of K or V
 constexpr int rows_lds(int waves) { return waves * 2 * RSLOT; }
 constexpr int kRowsGroups = 512;            // of 4 waves, two a CU; half as many of 8 waves
-constexpr int kMinShare = 2;                // blocks a share holds at least
+// Blocks a share holds at least. 1, 2, 3: 19.1, 13.1, 13.5 us for 4099 keys of one KV head
+// (one: 33 pieces), 17.8, 16.8, 17.6 for 8 requests of a window of 1024 keys and 8 heads.
+constexpr int kMinShare = 2;
 constexpr int DESC_INTS = 8;                // ints of a descriptor
 
 template <bool PAGED>
@@ -818,9 +822,11 @@ fa_serve_rows_kernel(AttnArgs a) {
 // 8 rows at once; up to kSomePieces the workgroup takes a row, 8 groups of 32 lanes
 // reading an 8th of the pieces each; beyond, a quarter of a row, 32 groups of 8 lanes.
 // So every workgroup has one row or quarter to join at most, and all its loads are in
-// flight at once: 34 pieces of 12 rows MIDDLE us, in quarters (which are 48 then) 10; 512
-// pieces of 12 rows in quarters 6.9, as the few are 23.6; 17 pieces as the few 4, in
-// quarters 16.
+// flight at once. Both launches for 8400 keys of 12 rows (33 pieces) take 12.1 us, with
+// quarters (of which there are 48) 20.0; for 4000 keys (16 pieces) 12.6, a row a workgroup
+// 13.4; for 131072 keys (512 pieces) 22.0, of which the join in quarters has 5, where
+// the first form alone took 23.6. The launch is short, so the length of its code counts:
+// expf instead of exp2, unrolled, cost 4 us at 64000 keys (18.5, not 14.7).
 constexpr int kFewPieces = 32, MERGE_EACH = 16, kSomePieces = 8 * MERGE_EACH;
 static_assert(32 * MERGE_EACH >= kRowsGroups, "every piece has a load");
 // e^(x - M), 0 for a part that saw no key (also where M is -inf). The product with log2 e
@@ -972,6 +978,11 @@ __device__ __forceinline__ void merge_rows(const AttnArgs& a, int block) {
 // With fewer tiles than CUs (a chunk behind a long cache) the lists of blocks are
 // cut into parts, a workgroup each, joined by a merge kernel. The lengths are
 // known on the GPU alone, so it decides there.
+//
+// Measured: a block of 128 keys takes a CU 3.6 us with all of them busy (16.8 MFLOP each,
+// 1190 TFLOP/s: the board's power limit; 3.1 in short launches), a tile 6.5 us besides (start,
+// first loads, stores). 32768 tokens of 12 heads, a window of 4096: 745 us, 1040
+// TFLOP/s of visible scores; 2048 tokens behind 30001, 12 heads: 391 us, 1000 TFLOP/s.
 constexpr int TT = 256;                     // rows of a tile
 constexpr int TTHREADS = 512;
 constexpr int TBLOCK = BLOCK * ROW_BYTES;   // bytes of a K or V block
@@ -979,7 +990,7 @@ constexpr int kTileLds = 4 * TBLOCK;
 constexpr int kTileItems = 512;             // parts of a launch that cuts tiles, at most
 constexpr int kTileGroups = 256;            // CUs: launches of fewer tiles may cut them
 constexpr int kCuts = 24;                   // parts of the longest tile, at most
-// Costs in units of a key block (3.5 us on a CU): what an item takes besides its
+// Costs in units of a key block (3.6 us on a CU): what an item takes besides its
 // blocks if it is a whole tile, or a part (256 rows of FP32 O to write), a merge
 // kernel, and every part's share of it (128 KiB to read).
 constexpr float kWholeCost = 2.f, kPartCost = 5.f, kMergeCost = 2.f, kMergeShare = 0.014f;
@@ -1522,7 +1533,7 @@ __device__ __forceinline__ Item find_item(const AttnArgs& a, const Dies& d, uint
 
 // In a mixed launch the workgroups from a.tile_groups on do the row kernel's work, in
 // 8 waves: they fill the CUs that have no long tile (22 decoding requests beside two
-// chunks of 1000 tokens: 193 us, one kernel after the other 214).
+// chunks of 1000 tokens: 136 us, one kernel after the other 166).
 template <bool BF, bool PAGED, bool MIXED>
 __global__ void __launch_bounds__(TTHREADS) __attribute__((amdgpu_waves_per_eu(2, 2)))
 fa_serve_tiles_kernel(AttnArgs a) {
@@ -1552,7 +1563,8 @@ fa_serve_tiles_kernel(AttnArgs a) {
   tile_item<BF, PAGED>(a, it, lds, &flag);
 }
 
-// Joins the parts of the tiles, 8 rows a workgroup, 32 lanes a row (4 dims each).
+// Joins the parts of the tiles, 8 rows a workgroup, 32 lanes a row (4 dims each). Bound by
+// memory: 480 parts of 96 tiles (63 MB) 17 us, 3.7 TB/s.
 template <bool BF, bool PAGED>
 __device__ __forceinline__ void merge_tiles(const AttnArgs& a, int block) {
   const int t = block >> 5;

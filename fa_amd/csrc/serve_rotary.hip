@@ -13,6 +13,8 @@
 // pieces: the dims of thread j's 8 pairs are dims 8j .. and rotary/2 + 8j ..
 // (halves) or 16j .. 16j + 15 (interleaved). The 8 angles of a thread depend on
 // the token alone, so with many tokens a thread keeps them for several heads.
+// 40007 tokens of 32 + 2 x 8 heads (984 MB) take 214 us, 4.6 TB/s, a large copy's
+// rate; 48 tokens 3.4 us, the launch.
 
 #include "serve_common.h"
 
@@ -122,7 +124,9 @@ __global__ void __launch_bounds__(ROTARY_THREADS) fa_serve_rotary_kernel(RotaryA
   }
 }
 
-// Threads a launch should have before a thread takes more than one head.
+// Threads a launch should have before a thread takes more than one head. With one, 16 and
+// this number of heads a thread (12 + 2 heads or 32 + 16): 300 tokens 4.0, 8.4 and 4.1 us;
+// 8000 tokens 14.6, 14.0 and 12.2; 40007 tokens of 48 heads 227, 216 and 215.
 constexpr int64_t ROTARY_WIDE = 256 * 1024;
 
 }  // namespace
