@@ -980,8 +980,8 @@ __device__ __forceinline__ void merge_rows(const AttnArgs& a, int block) {
 // known on the GPU alone, so it decides there.
 //
 // Measured: a block of 128 keys takes a CU 3.6 us with all of them busy (16.8 MFLOP each,
-// 1190 TFLOP/s: the board's power limit; 3.1 in short launches), a tile 6.5 us besides (start,
-// first loads, stores). 32768 tokens of 12 heads, a window of 4096: 745 us, 1040
+// 1190 TFLOP/s: the board's power limit; 3.1 in short launches), a tile 8 us besides: 2.5 until
+// it starts after the one before, 4.5 for its first loads, 1 for its stores. 32768 tokens of 12 heads, a window of 4096: 745 us, 1040
 // TFLOP/s of visible scores; 2048 tokens behind 30001, 12 heads: 391 us, 1000 TFLOP/s.
 constexpr int TT = 256;                     // rows of a tile
 constexpr int TTHREADS = 512;
@@ -1345,12 +1345,24 @@ __device__ __forceinline__ void tile_item(const AttnArgs& a, const Item& it, cha
       for (int e = 0; e < 4; ++e) out[e] = narrow<BF>(acc[dt][4 * g + e] * inv);
       *reinterpret_cast<u16x4*>(turn + l32 * ROW_BYTES + (((4 * dt + g) ^ (l32 & 15)) << 4) + hf * 8) = out;
     }
+  // All reads before the stores, which a branch each would keep apart (0.85 us a tile, not 1.5).
+  u32x4 val[8];
+  uint32_t lo[8], hi[8];
 #pragma unroll
   for (int x = 0; x < 8; ++x) {
     const int n = 4 * x + lr;
-    const u32x4 val = *reinterpret_cast<const u32x4*>(turn + n * ROW_BYTES + (((lane & 15) ^ (n & 15)) << 4));
-    const int64_t dst = (int64_t)(uint32_t)__shfl((int)obase, n) | (int64_t)__shfl((int)(obase >> 32), n) << 32;
-    if (row0 + n < rows && !(repaired >> n & 1)) *reinterpret_cast<u32x4*>(f.o + dst + (lane & 15) * 16) = val;
+    val[x] = *reinterpret_cast<const u32x4*>(turn + n * ROW_BYTES + (((lane & 15) ^ (n & 15)) << 4));
+    lo[x] = (uint32_t)__shfl((int)obase, n);
+    hi[x] = (uint32_t)__shfl((int)(obase >> 32), n);
+  }
+#pragma unroll
+  for (int x = 0; x < 8; ++x) asm volatile("" : "+v"(val[x]), "+v"(lo[x]), "+v"(hi[x]));
+  char* const out = f.o + (lane & 15) * 16;
+#pragma unroll
+  for (int x = 0; x < 8; ++x) {
+    const int n = 4 * x + lr;
+    const int64_t dst = (int64_t)(lo[x] | (uint64_t)hi[x] << 32);
+    if (row0 + n < rows && !(repaired >> n & 1)) *reinterpret_cast<u32x4*>(out + dst) = val[x];
   }
 }
 
