@@ -156,6 +156,27 @@ def test_a_nan_score_in_one_of_many_pieces(lib, spans, heads):
     assert o[own].isnan().all() and lse[own].isnan().all()
 
 
+# Which kernel, how many pieces.
+
+@pytest.mark.parametrize("keys", [8192, 8193, 32768, 32769, 131072])
+@pytest.mark.parametrize("heads", [(12, 1), (31, 1)])
+def test_joins_of_every_size(lib, keys, heads):
+    # One request: 32, 33, 128, 129 and 512 shares.
+    batch = Batch([(keys - 1, 1)], heads, 256, "fp16", seed=12)
+    o, lse = run(batch, lib)
+    batch.check(o, lse)
+
+
+@pytest.mark.parametrize("requests", [3, 11])
+@pytest.mark.parametrize("longest", [8, 9])
+def test_two_row_tiles_a_request(lib, requests, longest):
+    # Up to 64 rows a KV head, and 72, in launches of few and of more row tiles.
+    spans = [(150 + 97 * i, 1 + (longest - 1) * (i % 3) // 2) for i in range(requests)]
+    batch = Batch(spans, (64, 8), 32, "bf16", seed=13)
+    o, lse = run(batch, lib)
+    batch.check(o, lse)
+
+
 # Lengths, tables, padding.
 
 def test_rows_without_keys_and_empty_requests(lib):
