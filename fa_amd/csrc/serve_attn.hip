@@ -1495,8 +1495,13 @@ __device__ __forceinline__ Item find_item(const AttnArgs& a, const Dies& d, uint
       }
       __syncthreads();
       int best = 1;
-      for (int p = 2; p <= kCuts; ++p)
-        if (costs[p - 1] < costs[best - 1]) best = p;
+      float least = costs[0];
+#pragma unroll
+      for (int p = 2; p <= kCuts; ++p) {    // unrolled: its reads do not wait for each other
+        const float x = costs[p - 1];
+        best = x < least ? p : best;
+        least = x < least ? x : least;
+      }
       if (best > 1) length = cut_length(best, longest);
     }
     const bool cut = length < kUncut;
