@@ -1455,8 +1455,10 @@ __device__ __forceinline__ Item find_item(const AttnArgs& a, const Dies& d, uint
     // whole ones before this thread's run of requests.
     uint32_t tiles_mine = 0, whole_mine = 0;
     int2* const loads = reinterpret_cast<int2*>(lds);   // of every request: tiles, blocks
+    Request own{};                          // of request b0
     for (int b = b0; b < b1; ++b) {
       const Request r = request<PAGED>(a, b);
+      if (b == b0) own = r;
       const int tiles = tile_count<PAGED>(a, r), n = tiles ? tile_blocks(a, r) : 0;
       tiles_mine += min((int64_t)a.heads_kv * tiles, (int64_t)kTileGroups);
       whole_mine += tiles ? d.items_of(b, tiles) : 0;
@@ -1525,8 +1527,9 @@ __device__ __forceinline__ Item find_item(const AttnArgs& a, const Dies& d, uint
     if (x >= total) return none;            // uniform
     if (before <= x && x - before < mine) {
       uint32_t rel = x - before;
+      Request r = own;
       for (int b = b0; b < b1; ++b) {
-        const Request r = request<PAGED>(a, b);
+        if (b > b0) r = request<PAGED>(a, b);
         const int tiles = tile_count<PAGED>(a, r);
         if (!tiles) continue;
         const int parts = cut ? (loads[b].y + length - 1) / length : 1;
